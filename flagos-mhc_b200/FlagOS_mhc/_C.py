@@ -81,7 +81,28 @@ _SIGS = {
     "mhc_pre_bwd_accumulate": (ctypes.c_int, [_vp, _fp, _fp, _fp, _fp, _fp, _fp, _vp, _fp, _fp,
                                               _i64, _i32, _i64, _i32, _f32, _f32, _f32, _f32,
                                               _i32, _vp, _vp, _fp, _fp, _fp, _vp, _sz, _vp]),
+    "mhc_layer_norm_fwd": (ctypes.c_int, [_vp, _i64, _fp, _fp, _i64, _i64, _i32, _f32, _vp, _fp,
+                                          _fp, _vp]),
+    "mhc_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i32]),
+    "mhc_layer_norm_bwd": (ctypes.c_int, [_vp, _i64, _fp, _fp, _fp, _vp, _i64, _i64, _i64, _i32,
+                                          _vp, _fp, _fp, _vp, _sz, _vp]),
+    "mhc_linear_fwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "mhc_linear_fwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
+                                      _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
+    "mhc_linear_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32, _i32]),
+    "mhc_linear_bwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64,
+                                      _i64, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mhc_gated_ffn_fwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "mhc_gated_ffn_fwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64,
+                                         _i64, _i32, _i32, _vp, _vp, _vp, _i64, _vp, _sz, _vp]),
+    "mhc_gated_ffn_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "mhc_gated_ffn_bwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
+                                         _i64, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _vp,
+                                         _vp, _vp, _vp, _sz, _vp]),
 }
+
+# activations of the linear layer and the gated feed-forward block (enum mhc_act)
+_ACT = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
 def lib_path() -> str:
@@ -166,3 +187,48 @@ def require_cuda(*tensors):
         if t is not None and not t.is_cuda:
             raise RuntimeError("FlagOS_mhc: operators run only on CUDA (sm_100) tensors; "
                                f"got a tensor on {t.device}")
+
+
+def require_same(what, x, *others):
+    """The other tensors of a call: x's device and dtype (None is skipped)."""
+    for t in others:
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise RuntimeError(f"FlagOS_mhc.{what}: tensors on {x.device} and {t.device}")
+        if t.dtype != x.dtype:
+            raise ValueError(f"FlagOS_mhc.{what}: dtypes {x.dtype} and {t.dtype} in one call")
+
+
+def act_code(name):
+    try:
+        return _ACT[name]
+    except KeyError:
+        raise ValueError(f"FlagOS_mhc: unknown activation {name!r}; expected one of "
+                         f"{sorted(_ACT)}")
+
+
+def rows(t, width):
+    """(tensor, row stride in elements) of t = (T, width) or (B, S, width), read in place if its
+    rows share one stride, packed first otherwise."""
+    ts = token_view(t, 1, width)
+    if ts is None:
+        return t.contiguous(), width
+    return t, ts
+
+
+def unaligned(*pairs):
+    """1 if any (matrix, row stride) does not start its rows on 16-byte boundaries, else 0
+    (2-byte elements)."""
+    for t, ld in pairs:
+        if (t.data_ptr() | (ld << 1)) & 15:
+            return 1
+    return 0
+
+
+def workspace(nbytes, device):
+    """(tensor or None, pointer): torch's allocations are 512-byte aligned."""
+    if nbytes == 0:
+        return None, None
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, ptr(t)

@@ -6,7 +6,14 @@ saved tensors, same defaults).
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
+from .mhc_gated_ffn import mhc_gated_ffn
+from .mhc_gated_ffn_backward import mhc_gated_ffn_backward
+from .mhc_layer_norm import mhc_layer_norm
+from .mhc_layer_norm_backward import mhc_layer_norm_backward
+from .mhc_linear import mhc_linear
+from .mhc_linear_backward import mhc_linear_backward
 from .mhc_post import mhc_post
 from .mhc_post_backward import mhc_post_backward
 from .mhc_pre_clamp_sinkhorn import mhc_pre_clamp_sinkhorn
@@ -101,3 +108,77 @@ def mhc_pre_clamp_sinkhorn_fn(x, phi, alpha, base, norm_eps=1e-6, hc_eps=1e-6, c
     ``mhc_post_fn(..., next_phi=phi)`` returned with x."""
     return MhcPreClampSinkhornFn.apply(x, phi, alpha, base, norm_eps, hc_eps, clamp_min,
                                        clamp_max, iter_times, materialize_x_scaled, premix)
+
+
+class MhcLayerNormFn(torch.autograd.Function):
+    """Layer norm; saves (x, weight, mean, rstd)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        out = mhc_layer_norm(x, weight, bias, eps=eps, need_backward=True)
+        ctx.save_for_backward(x, weight, out["mean"], out["rstd"])
+        ctx.bias_dtype = bias.dtype if bias is not None else None
+        return out["y"]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        x, weight, mean, rstd = ctx.saved_tensors
+        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        gx, gw, gb = mhc_layer_norm_backward(x, weight, mean, rstd, grad_y,
+                                             need_param_grads=need_w or need_b)
+        return (gx, gw.to(weight.dtype) if need_w else None,
+                gb.to(ctx.bias_dtype) if need_b else None, None)
+
+
+def mhc_layer_norm_fn(x, weight=None, bias=None, eps=1e-5):
+    """Autograd-aware mhc_layer_norm. Returns y."""
+    return MhcLayerNormFn.apply(x, weight, bias, eps)
+
+
+class MhcLinearFn(torch.autograd.Function):
+    """Linear layer; saves (x, weight, z)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        out = mhc_linear(x, weight, bias=bias, residual=residual, activation=activation,
+                         need_backward=True)
+        ctx.save_for_backward(x, weight, out["z"])
+        ctx.activation = activation
+        return out["y"]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        x, weight, z = ctx.saved_tensors
+        nx, nw, nb, nr = ctx.needs_input_grad[:4]
+        gx, gw, gb = mhc_linear_backward(x, weight, z, grad_y, activation=ctx.activation,
+                                         need_x_grad=nx, need_weight_grad=nw, need_bias_grad=nb)
+        return gx, gw, gb, grad_y if nr else None, None
+
+
+def mhc_linear_fn(x, weight, bias=None, residual=None, activation="none"):
+    """Autograd-aware mhc_linear. Returns y."""
+    return MhcLinearFn.apply(x, weight, bias, residual, activation)
+
+
+class MhcGatedFfnFn(torch.autograd.Function):
+    """Gated feed-forward block; saves (x, w_gate, w_up, w_down, gate, up)."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation):
+        out = mhc_gated_ffn(x, w_gate, w_up, w_down, activation=activation, need_backward=True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, out["gate"], out["up"])
+        ctx.activation = activation
+        return out["y"]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        return mhc_gated_ffn_backward(*ctx.saved_tensors, grad_y, activation=ctx.activation,
+                                      need_grads=ctx.needs_input_grad[:4]) + (None,)
+
+
+def mhc_gated_ffn_fn(x, w_gate, w_up, w_down, activation="silu"):
+    """Autograd-aware mhc_gated_ffn. Returns y."""
+    return MhcGatedFfnFn.apply(x, w_gate, w_up, w_down, activation)

@@ -70,7 +70,7 @@ int sm_count() {
   return g_sms[dev];
 }
 
-static int check_device() {
+int check_device() {
   pdl_new_call();
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return MHC_ERR_CUDA;

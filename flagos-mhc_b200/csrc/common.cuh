@@ -371,6 +371,9 @@ inline cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
     default: return MHC_ERR_UNSUPPORTED_N;                   \
   }
 
+// MHC_OK on an sm_100 device, else MHC_ERR_DEVICE / MHC_ERR_CUDA; starts a new call for
+// the PDL rule above.
+int check_device();
 int sm_count();  // multiprocessors of the current device (cached per device)
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }

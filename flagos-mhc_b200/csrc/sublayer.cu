@@ -1,0 +1,337 @@
+// sublayer.cu -- entry points of the linear layer and the gated feed-forward block: argument
+// checks, workspace layout and the sequence of matrix products (gemm.cuh).
+#include "gemm.cuh"
+
+namespace mhc {
+
+// ------------------------------------------------------------------ gz and grad_bias
+// gz = grad_y * act'(z) in dtype and, per row range, the column sums of the unrounded gz.
+static constexpr int kGzRanges = 64;
+static int gz_ranges(int64_t T) { return (int)(T < kGzRanges * 64 ? cdiv(T, 64) : kGzRanges); }
+
+template <typename E, int ACT>
+__global__ void __launch_bounds__(256)
+    act_bwd_kernel(const E* __restrict__ z, int64_t zs, const E* __restrict__ gy, int64_t gs,
+                   int64_t T, int64_t F, E* __restrict__ gz, int64_t ld, float* __restrict__ part) {
+  pdl_enter();
+  const int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (f >= F) return;
+  const int64_t t0 = T * blockIdx.y / gridDim.y, t1 = T * (blockIdx.y + 1) / gridDim.y;
+  float s = 0.f;
+  for (int64_t t = t0; t < t1; ++t) {
+    float v = ld1<E>(gy + t * gs + f);
+    if constexpr (ACT != MHC_ACT_NONE) {
+      float a, da;
+      act_both<ACT>(ld1<E>(z + t * zs + f), a, da);
+      v *= da;
+    }
+    if (gz) st1<E>(gz + t * ld + f, v);
+    s += v;
+  }
+  if (part) part[(int64_t)blockIdx.y * F + f] = s;
+}
+
+template <typename E>
+__global__ void __launch_bounds__(256)
+    bias_finish_kernel(const float* __restrict__ part, int ranges, int64_t F, E* __restrict__ gb) {
+  pdl_enter();
+  const int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (f >= F) return;
+  Kahan k;
+  for (int i = 0; i < ranges; ++i) k.add(part[(int64_t)i * F + f]);
+  st1<E>(gb + f, k.s);
+}
+
+template <typename E>
+static int act_bwd_run(int act, const void* z, int64_t zs, const void* gy, int64_t gs, int64_t T,
+                       int64_t F, void* gz, int64_t ld, void* gb, float* part, cudaStream_t s) {
+  const int ranges = gz_ranges(T);
+  const dim3 grid((unsigned)cdiv(F, 256), ranges);
+  float* pt = gb ? part : nullptr;
+#define MHC_GZ(A)                                                                              \
+  (launch(act_bwd_kernel<E, A>, grid, 256, 0, s, (const E*)z, zs, (const E*)gy, gs, T, F, (E*)gz, \
+          ld, pt),                                                                              \
+   MHC_OK)
+  auto run = [&]() -> int { MHC_DISPATCH_ACT(act, MHC_GZ) };
+#undef MHC_GZ
+  const int st = run();
+  if (st != MHC_OK) return st;
+  MHC_LAUNCH_CHECK();
+  if (gb) {
+    launch(bias_finish_kernel<E>, (unsigned)cdiv(F, 256), 256, 0, s, (const float*)part, ranges, F,
+           (E*)gb);
+    MHC_LAUNCH_CHECK();
+  }
+  return MHC_OK;
+}
+
+// ------------------------------------------------------------------ checks and workspace
+static int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
+static int sub_check(int64_t T, int64_t D, int64_t F, int32_t dtype, int32_t act) {
+  // tile coordinates are 32-bit
+  if (T < 0 || D <= 0 || F <= 0 || T > INT32_MAX - 512 || D > INT32_MAX / 8 || F > INT32_MAX / 8)
+    return MHC_ERR_INVALID_ARGUMENT;
+  if (dtype != MHC_F16 && dtype != MHC_BF16) return MHC_ERR_UNSUPPORTED_DTYPE;
+  if (act < MHC_ACT_NONE || act > MHC_ACT_SILU) return MHC_ERR_INVALID_ARGUMENT;
+  return MHC_OK;
+}
+
+static bool ws_ok(const void* ws, size_t bytes, size_t need) {
+  return need == 0 || (ws && bytes >= need && (reinterpret_cast<uintptr_t>(ws) & 255) == 0);
+}
+
+// Takes regions of the workspace in order; with a null base only the offsets are counted.
+struct Carver {
+  char* base;
+  size_t off = 0;
+  void* take(size_t bytes) {
+    void* p = base ? base + off : nullptr;
+    off += align_up(bytes);
+    return p;
+  }
+};
+
+static int zero(void* p, size_t bytes, cudaStream_t s) {
+  if (p && bytes) MHC_CUDA_CHECK(cudaMemsetAsync(p, 0, bytes, s));
+  return MHC_OK;
+}
+
+}  // namespace mhc
+
+using namespace mhc;
+
+#define RETURN_IF(x)               \
+  do {                             \
+    int _st = (x);                 \
+    if (_st != MHC_OK) return _st; \
+  } while (0)
+
+extern "C" {
+
+size_t mhc_linear_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
+                                      int32_t unaligned) {
+  (void)unaligned;
+  if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
+  return 0;
+}
+
+int mhc_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                   const void* bias, const void* residual, int64_t residual_stride, int64_t T,
+                   int64_t D, int64_t F, int32_t dtype, int32_t act, void* y, void* z,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  RETURN_IF(sub_check(T, D, F, dtype, act));
+  if (x_stride < D || weight_stride < D || (residual && residual_stride < F))
+    return MHC_ERR_INVALID_ARGUMENT;
+  if (T == 0) return MHC_OK;
+  if (!x || !weight || !y) return MHC_ERR_INVALID_ARGUMENT;
+  if (!ws_ok(workspace, workspace_bytes, mhc_linear_fwd_workspace_bytes(T, D, F, dtype, 0)))
+    return MHC_ERR_WORKSPACE;
+  RETURN_IF(check_device());
+  Gemm g;
+  g.dtype = dtype;
+  g.M = T; g.N = F; g.K = D;
+  g.a = {x, x_stride, true};
+  g.b = {weight, weight_stride, true};
+  g.epi.act = act; g.epi.out = y; g.epi.ld_out = F; g.epi.bias = bias; g.epi.z = z;
+  g.epi.res = residual; g.epi.ld_res = residual ? residual_stride : 0;
+  return gemm_run(g, (cudaStream_t)stream);
+}
+
+size_t mhc_linear_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
+                                      int32_t act, int32_t unaligned) {
+  (void)unaligned;
+  if (sub_check(T, D, F, dtype, act) != MHC_OK) return 0;
+  Carver c{nullptr};
+  if (act != MHC_ACT_NONE) c.take((size_t)T * pad8(F) * 2);
+  c.take((size_t)gz_ranges(T) * F * 4);
+  return c.off;
+}
+
+int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                   const void* z, int64_t z_stride, const void* grad_y, int64_t grad_y_stride,
+                   int64_t T, int64_t D, int64_t F, int32_t dtype, int32_t act, void* grad_x,
+                   void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+  RETURN_IF(sub_check(T, D, F, dtype, act));
+  if (x_stride < D || weight_stride < D || grad_y_stride < F ||
+      (act != MHC_ACT_NONE && z_stride < F))
+    return MHC_ERR_INVALID_ARGUMENT;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (T > 0 && (!x || !weight || !grad_y || (act != MHC_ACT_NONE && !z)))
+    return MHC_ERR_INVALID_ARGUMENT;
+  if (T > 0 && !ws_ok(workspace, workspace_bytes,
+                      mhc_linear_bwd_workspace_bytes(T, D, F, dtype, act, 0)))
+    return MHC_ERR_WORKSPACE;
+  RETURN_IF(check_device());
+  if (T == 0) {
+    RETURN_IF(zero(grad_weight, (size_t)F * D * 2, s));
+    return zero(grad_bias, (size_t)F * 2, s);
+  }
+  Carver c{(char*)workspace};
+  void* gzb = act != MHC_ACT_NONE ? c.take((size_t)T * pad8(F) * 2) : nullptr;
+  float* part = (float*)c.take((size_t)gz_ranges(T) * F * 4);
+  if (gzb || grad_bias) {
+    const int64_t ld = pad8(F);
+    RETURN_IF(dtype == MHC_F16
+                  ? act_bwd_run<__half>(act, z, z_stride, grad_y, grad_y_stride, T, F, gzb, ld,
+                                        grad_bias, part, s)
+                  : act_bwd_run<__nv_bfloat16>(act, z, z_stride, grad_y, grad_y_stride, T, F, gzb,
+                                               ld, grad_bias, part, s));
+  }
+  const void* gz = gzb ? gzb : grad_y;
+  const int64_t gzs = gzb ? pad8(F) : grad_y_stride;
+  Gemm g;
+  g.dtype = dtype;
+  if (grad_x) {
+    g.M = T; g.N = D; g.K = F;
+    g.a = {gz, gzs, true};
+    g.b = {weight, weight_stride, false};
+    g.epi.out = grad_x; g.epi.ld_out = D;
+    RETURN_IF(gemm_run(g, s));
+  }
+  if (grad_weight) {
+    g.M = F; g.N = D; g.K = T;
+    g.a = {gz, gzs, false};
+    g.b = {x, x_stride, false};
+    g.epi.out = grad_weight; g.epi.ld_out = D;
+    RETURN_IF(gemm_run(g, s));
+  }
+  return MHC_OK;
+}
+
+size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
+                                         int32_t unaligned) {
+  (void)unaligned;
+  if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
+  Carver c{nullptr};
+  c.take((size_t)T * pad8(F) * 2);  // h
+  return c.off;
+}
+
+int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride,
+                      const void* w_up, int64_t w_up_stride, const void* w_down,
+                      int64_t w_down_stride, int64_t T, int64_t D, int64_t F, int32_t dtype,
+                      int32_t act, void* y, void* gate, void* up, int64_t gate_up_stride,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  RETURN_IF(sub_check(T, D, F, dtype, act));
+  if (x_stride < D || w_gate_stride < D || w_up_stride < D || w_down_stride < F ||
+      (gate == nullptr) != (up == nullptr) || (gate && gate_up_stride < F))
+    return MHC_ERR_INVALID_ARGUMENT;
+  if (T == 0) return MHC_OK;
+  if (!x || !w_gate || !w_up || !w_down || !y) return MHC_ERR_INVALID_ARGUMENT;
+  if (!ws_ok(workspace, workspace_bytes, mhc_gated_ffn_fwd_workspace_bytes(T, D, F, dtype, 0)))
+    return MHC_ERR_WORKSPACE;
+  RETURN_IF(check_device());
+  const cudaStream_t s = (cudaStream_t)stream;
+  Carver c{(char*)workspace};
+  const int64_t ldh = pad8(F);
+  void* h = c.take((size_t)T * ldh * 2);
+  Gemm g;
+  g.kind = kEpiGated;
+  g.dtype = dtype;
+  g.M = T; g.N = F; g.K = D;
+  g.a = {x, x_stride, true};
+  g.b = {w_gate, w_gate_stride, true};
+  g.b2 = {w_up, w_up_stride, true};
+  g.epi.act = act; g.epi.out = h; g.epi.ld_out = ldh;
+  g.epi.gate = gate; g.epi.up = up; g.epi.ld_gu = gate ? gate_up_stride : 0;
+  RETURN_IF(gemm_run(g, s));
+  Gemm d;
+  d.dtype = dtype;
+  d.M = T; d.N = D; d.K = F;
+  d.a = {h, ldh, true};
+  d.b = {w_down, w_down_stride, true};
+  d.epi.out = y; d.epi.ld_out = D;
+  return gemm_run(d, s);
+}
+
+size_t mhc_gated_ffn_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
+                                         int32_t unaligned) {
+  (void)unaligned;
+  if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
+  Carver c{nullptr};
+  for (int i = 0; i < 3; ++i) c.take((size_t)T * pad8(F) * 2);  // gg, gu, h
+  return c.off;
+}
+
+int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride,
+                      const void* w_up, int64_t w_up_stride, const void* w_down,
+                      int64_t w_down_stride, const void* gate, const void* up,
+                      int64_t gate_up_stride, const void* grad_y, int64_t grad_y_stride,
+                      int64_t T, int64_t D, int64_t F, int32_t dtype, int32_t act, void* grad_x,
+                      void* grad_w_gate, void* grad_w_up, void* grad_w_down, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  RETURN_IF(sub_check(T, D, F, dtype, act));
+  if (x_stride < D || w_gate_stride < D || w_up_stride < D || w_down_stride < F ||
+      gate_up_stride < F || grad_y_stride < D)
+    return MHC_ERR_INVALID_ARGUMENT;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (T > 0 && (!x || !w_gate || !w_up || !w_down || !gate || !up || !grad_y))
+    return MHC_ERR_INVALID_ARGUMENT;
+  if (T > 0 && !ws_ok(workspace, workspace_bytes,
+                      mhc_gated_ffn_bwd_workspace_bytes(T, D, F, dtype, 0)))
+    return MHC_ERR_WORKSPACE;
+  RETURN_IF(check_device());
+  if (T == 0) {
+    RETURN_IF(zero(grad_w_gate, (size_t)F * D * 2, s));
+    RETURN_IF(zero(grad_w_up, (size_t)F * D * 2, s));
+    return zero(grad_w_down, (size_t)F * D * 2, s);
+  }
+  Carver c{(char*)workspace};
+  const int64_t ld = pad8(F);
+  void* gg = c.take((size_t)T * ld * 2);
+  void* gu = c.take((size_t)T * ld * 2);
+  void* h = c.take((size_t)T * ld * 2);
+  {
+    Gemm g;  // gh = grad_y w_down, then gg, gu and h in its epilogue
+    g.kind = kEpiGatedBwd;
+    g.dtype = dtype;
+    g.M = T; g.N = F; g.K = D;
+    g.a = {grad_y, grad_y_stride, true};
+    g.b = {w_down, w_down_stride, false};
+    g.epi.act = act;
+    g.epi.gate = const_cast<void*>(gate); g.epi.up = const_cast<void*>(up);
+    g.epi.ld_gu = gate_up_stride;
+    g.epi.gg = gg; g.epi.gu = gu; g.epi.ld_g = ld;
+    g.epi.out = h; g.epi.ld_out = ld;
+    RETURN_IF(gemm_run(g, s));
+  }
+  Gemm g;
+  g.dtype = dtype;
+  if (grad_x) {
+    g.M = T; g.N = D; g.K = F;
+    g.a = {gg, ld, true};
+    g.b = {w_gate, w_gate_stride, false};
+    g.a3 = {gu, ld, true};
+    g.b3 = {w_up, w_up_stride, false};
+    g.K3 = F;
+    g.epi.out = grad_x; g.epi.ld_out = D;
+    RETURN_IF(gemm_run(g, s));
+    g.K3 = 0;
+  }
+  g.K = T;
+  g.M = F; g.N = D;
+  g.b = {x, x_stride, false};
+  g.epi.ld_out = D;
+  if (grad_w_gate) {
+    g.a = {gg, ld, false};
+    g.epi.out = grad_w_gate;
+    RETURN_IF(gemm_run(g, s));
+  }
+  if (grad_w_up) {
+    g.a = {gu, ld, false};
+    g.epi.out = grad_w_up;
+    RETURN_IF(gemm_run(g, s));
+  }
+  if (grad_w_down) {
+    g.M = D; g.N = F;
+    g.a = {grad_y, grad_y_stride, false};
+    g.b = {h, ld, false};
+    g.epi.out = grad_w_down; g.epi.ld_out = F;
+    RETURN_IF(gemm_run(g, s));
+  }
+  return MHC_OK;
+}
+
+}  // extern "C"

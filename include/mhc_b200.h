@@ -315,6 +315,134 @@ int mhc_pre_fwd_noalloc(const void* x, const float* phi, const float* alpha,
                         float* inv_rms, float* x_scaled, float* mixes,
                         float* h_res_logits, float* pre, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Sublayer operators: what stands between a layer's pre operator (its y) and
+ * its post operator (h_out).  No counterpart in the reference.
+ *
+ * Rows (tokens) may be strided: *_stride is the number of elements between
+ * consecutive rows, the elements of a row are contiguous.  A matrix is
+ * "aligned" if its base is a multiple of 16 bytes and its row stride a multiple
+ * of 16 bytes; others are accepted and cost a packed copy in the workspace.
+ * The workspace queries take `unaligned`: 0 if every matrix operand (x, weights,
+ * grad_y) is aligned, 1 otherwise.  T = 0 is valid: parameter gradients are
+ * then zero.  MHC_F32 is taken by the layer norm only (the matrix products
+ * return MHC_ERR_UNSUPPORTED_DTYPE).  Sums are held in fp32 and added in a
+ * fixed order; each output is rounded once. */
+enum mhc_act {
+  MHC_ACT_NONE = 0,
+  MHC_ACT_RELU = 1,
+  MHC_ACT_GELU = 2,      /* z * Phi(z), by erf               */
+  MHC_ACT_GELU_TANH = 3, /* the tanh form of the same        */
+  MHC_ACT_SILU = 4       /* z * sigmoid(z)                   */
+};
+
+/*
+ * Layer norm forward over rows of D:
+ *   mean = sum(x)/D;  rstd = rsqrt(sum((x-mean)^2)/D + eps)
+ *   y = (x - mean) * rstd * weight + bias
+ * x: (T,D) dtype, rows x_stride apart.  weight, bias: (D,) fp32 or NULL (1, 0).
+ * y: (T,D) dtype, packed.  mean, rstd: (T,) fp32 or NULL.
+ */
+int mhc_layer_norm_fwd(const void* x, int64_t x_stride, const float* weight,
+                       const float* bias, int64_t T, int64_t D, int32_t dtype,
+                       float eps, void* y, float* mean, float* rstd,
+                       void* stream);
+
+/* Bytes of device workspace mhc_layer_norm_bwd needs. */
+size_t mhc_layer_norm_bwd_workspace_bytes(int64_t T, int64_t D, int32_t dtype);
+
+/*
+ * Layer norm backward, with h = grad_y * weight, xh = (x - mean) * rstd:
+ *   grad_x = rstd * (h - sum(h)/D - xh * sum(h*xh)/D)
+ *   grad_weight = sum_t grad_y * xh;  grad_bias = sum_t grad_y
+ * grad_x: (T,D) dtype, packed.  grad_weight, grad_bias: (D,) fp32, or NULL
+ * (both or neither).  workspace: 256-byte aligned, not needed when the two
+ * are NULL.
+ */
+int mhc_layer_norm_bwd(const void* x, int64_t x_stride, const float* weight,
+                       const float* mean, const float* rstd,
+                       const void* grad_y, int64_t grad_y_stride, int64_t T,
+                       int64_t D, int32_t dtype, void* grad_x,
+                       float* grad_weight, float* grad_bias, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace mhc_linear_fwd needs (may be 0). */
+size_t mhc_linear_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F,
+                                      int32_t dtype, int32_t unaligned);
+
+/*
+ * Linear layer with its epilogue:
+ *   z = x weight^T + bias;  y = act(z) + residual
+ * x: (T,D); weight: (F,D); bias: (F,) or NULL; residual: (T,F) or NULL;
+ * y: (T,F) packed; z: (T,F) packed or NULL (kept for the backward).  All dtype.
+ */
+int mhc_linear_fwd(const void* x, int64_t x_stride, const void* weight,
+                   int64_t weight_stride, const void* bias,
+                   const void* residual, int64_t residual_stride, int64_t T,
+                   int64_t D, int64_t F, int32_t dtype, int32_t act, void* y,
+                   void* z, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* Bytes of device workspace mhc_linear_bwd needs. */
+size_t mhc_linear_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F,
+                                      int32_t dtype, int32_t act,
+                                      int32_t unaligned);
+
+/*
+ * Linear backward:  gz = grad_y * act'(z)   (rounded to dtype: it is a matrix
+ * operand);  grad_x = gz weight;  grad_weight = gz^T x;  grad_bias = sum_t gz
+ * (from the unrounded gz).  z: (T,F) dtype, rows z_stride apart; NULL for
+ * MHC_ACT_NONE.  grad_x (T,D), grad_weight (F,D), grad_bias (F,): dtype, packed;
+ * each may be NULL and is then not computed.  The residual's gradient is grad_y.
+ */
+int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight,
+                   int64_t weight_stride, const void* z, int64_t z_stride,
+                   const void* grad_y, int64_t grad_y_stride, int64_t T,
+                   int64_t D, int64_t F, int32_t dtype, int32_t act,
+                   void* grad_x, void* grad_weight, void* grad_bias,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace mhc_gated_ffn_fwd needs. */
+size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F,
+                                         int32_t dtype, int32_t unaligned);
+
+/*
+ * Gated feed-forward block:
+ *   gate = x w_gate^T;  up = x w_up^T;  h = act(gate) * up;  y = h w_down^T
+ * x: (T,D); w_gate, w_up: (F,D); w_down: (D,F); y: (T,D) packed; gate, up:
+ * (T,F), rows gate_up_stride apart, or NULL (both or neither; kept for the
+ * backward).  All dtype.  h is rounded to dtype: it is a matrix operand.
+ */
+int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate,
+                      int64_t w_gate_stride, const void* w_up,
+                      int64_t w_up_stride, const void* w_down,
+                      int64_t w_down_stride, int64_t T, int64_t D, int64_t F,
+                      int32_t dtype, int32_t act, void* y, void* gate, void* up,
+                      int64_t gate_up_stride, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace mhc_gated_ffn_bwd needs. */
+size_t mhc_gated_ffn_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F,
+                                         int32_t dtype, int32_t unaligned);
+
+/*
+ * Gated feed-forward backward:
+ *   gh = grad_y w_down;  gg = gh * up * act'(gate);  gu = gh * act(gate)
+ *   grad_x = gg w_gate + gu w_up;  grad_w_gate = gg^T x;  grad_w_up = gu^T x
+ *   grad_w_down = grad_y^T h,  h = act(gate) * up
+ * gg, gu and h are rounded to dtype: they are matrix operands.  Outputs: dtype,
+ * packed; each may be NULL and is then not computed.
+ */
+int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate,
+                      int64_t w_gate_stride, const void* w_up,
+                      int64_t w_up_stride, const void* w_down,
+                      int64_t w_down_stride, const void* gate, const void* up,
+                      int64_t gate_up_stride, const void* grad_y,
+                      int64_t grad_y_stride, int64_t T, int64_t D, int64_t F,
+                      int32_t dtype, int32_t act, void* grad_x,
+                      void* grad_w_gate, void* grad_w_up, void* grad_w_down,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
