@@ -31,6 +31,7 @@ int post_mix_run(const void* x, const float* h_res, const void* h_out, const flo
                  void* out, int64_t T, int64_t D, int32_t dtype, const float* phi_next,
                  float* premix, int32_t layers, void* ws, cudaStream_t s);
 int tc_host_device_error();
+int gemm_device_error();
 
 static std::atomic<unsigned long long> g_launches{0};
 void note_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
@@ -146,7 +147,8 @@ int mhc_device_status(void) {
   const int e = tc_host_device_error();
   const int f = post_mix_device_error();
   const int g = pre_bwd_tc32_device_error();
-  const int all[7] = {a, b, c, d, e, f, g};
+  const int h = gemm_device_error();
+  const int all[8] = {a, b, c, d, e, f, g, h};
   for (int v : all)
     if (v != MHC_OK) return v;
   return MHC_OK;

@@ -1,55 +1,301 @@
-// gemm.cu -- matrix product with the operators' epilogues: 64 x 64 tiles in shared memory,
-// fp32 multiply-adds, a thread owns one row and 16 columns.
+// gemm.cu -- the matrix product of gemm.cuh on tcgen05, with the operators' epilogues.
+//
+// A cluster of two CTAs owns a 256 x 256 tile (cta_group::2): each CTA keeps 128 rows of A
+// and half of the tile's B rows per 64-deep K block in shared memory, and 128 x 256 fp32
+// accumulators in TMEM, of which there are two sets: the epilogue of one tile runs beside
+// the products of the next.  Warp 0 loads (TMA, 6 stages of 32 KB), one thread of the
+// leader CTA issues the MMAs of both, eight warps run the epilogue.  For the gated kinds of
+// product the leader's B rows are the gate projection's and its peer's the up projection's,
+// so both values of one hidden element meet in one thread.
+//
+// Either operand may be K-major or MN-major (the transposed products of the backward): only
+// the TMA box and the shared-memory descriptor differ.  Rows and columns past the edges are
+// read as zeros and not stored.
+#include <algorithm>
+
 #include "gemm.cuh"
+#include "tc.cuh"
 
 namespace mhc {
+namespace gk {
+constexpr int BM = 128;          // rows of A per CTA (256 per cluster)
+constexpr int BNC = 128;         // rows of B per CTA (256 per cluster)
+constexpr int BK = 64;
+constexpr int STAGES = 6;
+constexpr int A_BYTES = BM * BK * 2, B_BYTES = BNC * BK * 2;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int SMEM = STAGES * STAGE_BYTES + 1024;  // and room to align
+constexpr int GROUP_M = 8;       // row tiles that walk the column tiles together
+}  // namespace gk
 
-static constexpr int kBM = 64, kBN = 64, kBK = 16, kNC = 16;
+struct GemmMaps {
+  CUtensorMap a, b, b2, a3, b3;
+};
+// How one launch walks the problem.
+struct GemmWalk {
+  int64_t M, N;                       // of the output
+  int32_t tiles_m, tiles_n, nk1, nk;  // K blocks of the first segment, of both
+  int32_t a_k, b_k, a3_k, b3_k;       // operands that are K-major
+};
 
-template <typename E>
-__device__ __forceinline__ void load_tile(float (*s)[kBM + 1], const Operand& o, int64_t r0,
-                                          int64_t R, int64_t k0, int64_t K) {
-  const E* p = (const E*)o.p;
-  for (int i = threadIdx.x; i < kBM * kBK; i += 256) {
-    const int r = o.k_major ? i / kBK : i % kBM, k = o.k_major ? i % kBK : i / kBM;
-    float v = 0.f;
-    if (r0 + r < R && k0 + k < K)
-      v = from_e(p[o.k_major ? (r0 + r) * o.ld + k0 + k : (k0 + k) * o.ld + r0 + r]);
-    s[k][r] = v;
+namespace tc2 {
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// address of the leader CTA's copy of a shared variable
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(tc::smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// a third of a second at least; the longest healthy wait is one tile's products
+constexpr uint32_t kSpin = 1u << 24;
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  for (uint32_t i = 0; i < kSpin; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(tc::smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((i & 255) == 255 && *abort) return false;
   }
+  *abort = 1;
+  return false;
+}
+// load into this CTA's shared memory; the bytes are counted on the leader's barrier
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                        int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                    uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrive on this barrier of both CTAs once all MMAs issued so far have completed
+__device__ __forceinline__ void commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(tc::smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void ld32(uint32_t taddr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+}  // namespace tc2
+
+// tile index -> tile row and column: GROUP_M row tiles walk all column tiles together, so the
+// tiles in flight share their operands in L2
+__device__ __forceinline__ void tile_at(const GemmWalk& w, int32_t i, int32_t& mt, int32_t& nt) {
+  const int32_t per = gk::GROUP_M * w.tiles_n;
+  const int32_t g = i / per, rest = i - g * per;
+  const int32_t rows = min(gk::GROUP_M, w.tiles_m - g * gk::GROUP_M);
+  nt = rest / rows;
+  mt = g * gk::GROUP_M + rest - nt * rows;
 }
 
 template <typename E, int KIND>
-__global__ void __launch_bounds__(256) gemm_kernel(Gemm g) {
-  pdl_enter();
+__global__ void __launch_bounds__(gk::THREADS, 1)
+    gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmWalk w,
+                const __grid_constant__ EpiParams epi) {
+  using namespace gk;
   constexpr bool dual = KIND == kEpiGated;
-  __shared__ float sa[kBK][kBM + 1], sb[kBK][kBN + 1], sb2[dual ? kBK : 1][kBN + 1];
-  const int64_t m0 = (int64_t)blockIdx.x * kBM, n0 = (int64_t)blockIdx.y * kBN;
-  const int r = threadIdx.x & 63, c = (threadIdx.x >> 6) * kNC;
-  float acc[kNC] = {}, acc2[kNC] = {};
-  for (int seg = 0; seg < 2; ++seg) {
-    const Operand &A = seg ? g.a3 : g.a, &B = seg ? g.b3 : g.b;
-    const int64_t K = seg ? g.K3 : g.K;
-    for (int64_t k0 = 0; k0 < K; k0 += kBK) {
-      load_tile<E>(sa, A, m0, g.M, k0, K);
-      load_tile<E>(sb, B, n0, g.N, k0, K);
-      if constexpr (dual) load_tile<E>(sb2, g.b2, n0, g.N, k0, K);
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kBK; ++k) {
-        const float a = sa[k][r];
-#pragma unroll
-        for (int i = 0; i < kNC; ++i) {
-          acc[i] = fmaf(a, sb[k][c + i], acc[i]);
-          if constexpr (dual) acc2[i] = fmaf(a, sb2[k][c + i], acc2[i]);
+  extern __shared__ char smem_raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                       ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2], tdone;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = tc2::cta_rank();
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&tfull[i], 1);
+      tc::mbar_init(&tempty[i], 2 * EPI_WARPS);
+    }
+    tc::mbar_init(&tdone, 1);
+    abort_word = 0;
+    tc::fence_barrier_init();
+    tc::prefetch_tmap(&maps.a);
+    tc::prefetch_tmap(&maps.b);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     tc::smem_u32(&tmem_slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc2::cluster_sync();  // both CTAs' barriers are initialised
+  tc::tc_fence_after();
+  const uint32_t tmem = *(volatile uint32_t*)&tmem_slot;
+  pdl_enter();
+
+  const int32_t tiles = w.tiles_m * w.tiles_n;
+  const int32_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  if (warp == 0) {
+    // ---------------------------------------------------------------- loads
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int32_t i = first; i < tiles && ok; i += step) {
+        int32_t mt, nt;
+        tile_at(w, i, mt, nt);
+        const int32_t m0 = mt * 2 * BM + (int32_t)rank * BM;
+        const int32_t n0 = dual ? nt * BNC : nt * 2 * BNC + (int32_t)rank * BNC;
+        for (int32_t kb = 0; kb < w.nk; ++kb, ++it) {
+          const uint32_t s = it % STAGES;
+          if (!tc2::wait_cluster(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (leader) tc::mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
+          const uint32_t bar = tc2::leader_addr(&full[s]);
+          const uint32_t sa = tc::smem_u32(smem + s * STAGE_BYTES), sb = sa + A_BYTES;
+          const bool second = kb >= w.nk1;
+          const int32_t k0 = (second ? kb - w.nk1 : kb) * BK;
+          const CUtensorMap* ma = second ? &maps.a3 : &maps.a;
+          const CUtensorMap* mb = second ? &maps.b3 : (dual && rank) ? &maps.b2 : &maps.b;
+          if (second ? w.a3_k : w.a_k) {
+            tc2::load_2d(sa, ma, bar, k0, m0);
+          } else {
+            tc2::load_2d(sa, ma, bar, m0, k0);
+            tc2::load_2d(sa + A_BYTES / 2, ma, bar, m0 + 64, k0);
+          }
+          if (second ? w.b3_k : w.b_k) {
+            tc2::load_2d(sb, mb, bar, k0, n0);
+          } else {
+            tc2::load_2d(sb, mb, bar, n0, k0);
+            tc2::load_2d(sb + B_BYTES / 2, mb, bar, n0 + 64, k0);
+          }
         }
       }
-      __syncthreads();
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMAs
+    if (lane == 0) {
+      if (leader) {
+        // descriptor step of 16 K elements: 32 bytes of a K-major row, or two 8-row atoms
+        const uint32_t idesc1 = tc::idesc_16<E>(256, 256, !w.a_k, !w.b_k);
+        const uint32_t idesc2 = tc::idesc_16<E>(256, 256, !w.a3_k, !w.b3_k);
+        uint32_t it = 0, j = 0;
+        bool ok = true;
+        for (int32_t i = first; i < tiles && ok; i += step, ++j) {
+          const uint32_t buf = j & 1;
+          if (!tc2::wait_cluster(&tempty[buf], ((j >> 1) & 1) ^ 1, abort_flag)) break;
+          tc::tc_fence_after();
+          const uint32_t d = tmem + buf * 256;
+          for (int32_t kb = 0; kb < w.nk; ++kb, ++it) {
+            const uint32_t s = it % STAGES;
+            if (!tc2::wait_cluster(&full[s], (it / STAGES) & 1, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc::tc_fence_after();
+            const bool second = kb >= w.nk1;
+            const bool ak = second ? w.a3_k : w.a_k, bk = second ? w.b3_k : w.b_k;
+            const uint32_t sa = tc::smem_u32(smem + s * STAGE_BYTES);
+            const uint64_t da = tc::smem_desc(sa, ak ? 16 : A_BYTES / 2, 1024, tc::kSwizzle128);
+            const uint64_t db =
+                tc::smem_desc(sa + A_BYTES, bk ? 16 : B_BYTES / 2, 1024, tc::kSwizzle128);
+            const uint32_t stepa = ak ? 2 : 128, stepb = bk ? 2 : 128;
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+              tc2::mma(d, da + k * stepa, db + k * stepb, second ? idesc2 : idesc1,
+                       (kb != 0 || k != 0) ? 1u : 0u);
+            tc2::commit_both(&empty[s]);
+          }
+          if (!ok) break;
+          tc2::commit_both(&tfull[buf]);
+        }
+        tc2::commit_both(&tdone);  // every MMA has completed before TMEM is freed
+      }
+      volatile int never = 0;
+      tc2::wait_cluster(&tdone, 0, &never);
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    constexpr int COLS = dual ? BNC / 2 : BNC;  // output columns per warp
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t tq = tmem + ((uint32_t)(q * 32) << 16) + half * COLS;
+    uint32_t j = 0;
+    for (int32_t i = first; i < tiles; i += step, ++j) {
+      int32_t mt, nt;
+      tile_at(w, i, mt, nt);
+      const uint32_t buf = j & 1;
+      const bool got = tc2::wait_cluster(&tfull[buf], (j >> 1) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, got)) break;
+      tc::tc_fence_after();
+      const int64_t row = (int64_t)mt * 2 * BM + rank * BM + q * 32 + lane;
+      const int64_t col0 = (int64_t)nt * (dual ? BNC : 2 * BNC) + half * COLS;
+#pragma unroll 1
+      for (int c = 0; c < COLS; c += 32) {
+        __syncwarp();  // rows past M skip the epilogue below
+        float acc[32], acc2[dual ? 32 : 1];
+        tc2::ld32(tq + buf * 256 + c, acc);
+        if constexpr (dual) tc2::ld32(tq + buf * 256 + BNC + c, acc2);
+        tc::tmem_ld_wait();
+        if (c + 32 == COLS) {  // the accumulators have been read
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc2::arrive_cluster(tc2::leader_addr(&tempty[buf]));
+        }
+        const int64_t left = w.N - (col0 + c);
+        if (row < w.M && left > 0)
+          epi_chunk<E, KIND, 32>(epi, row, col0 + c, left < 32 ? (int)left : 32, acc, acc2);
+      }
     }
   }
-  const int64_t left = g.N - (n0 + c);
-  if (m0 + r < g.M && left > 0)
-    epi_chunk<E, KIND, kNC>(g.epi, m0 + r, n0 + c, left < kNC ? (int)left : kNC, acc, acc2);
+  __syncwarp();
+  if (*abort_flag && threadIdx.x == 0) flag_timeout();
+  tc::tc_fence_before();
+  __syncthreads();
+  tc2::cluster_sync();  // neither CTA leaves while the other may still signal it
+  if (warp == 1) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
 }
 
 bool epi_vec_ok(const Gemm& g) {
@@ -59,23 +305,118 @@ bool epi_vec_ok(const Gemm& g) {
          e.ld_gu % 8 == 0 && aligned16(e.gg) && aligned16(e.gu) && e.ld_g % 8 == 0;
 }
 
-template <typename E>
-static int gemm_typed(const Gemm& g, cudaStream_t s) {
-  const dim3 grid((unsigned)cdiv(g.M, kBM), (unsigned)cdiv(g.N, kBN));
-  if (g.kind == kEpiGated)
-    launch(gemm_kernel<E, kEpiGated>, grid, 256, 0, s, g);
-  else if (g.kind == kEpiGatedBwd)
-    launch(gemm_kernel<E, kEpiGatedBwd>, grid, 256, 0, s, g);
-  else
-    launch(gemm_kernel<E, kEpiLinear>, grid, 256, 0, s, g);
+bool operand_aligned(const Operand& o) { return aligned16(o.p) && o.ld % 8 == 0; }
+
+static int operand_map(CUtensorMap* m, const Operand& o, int32_t dtype, int64_t mn, int64_t k) {
+  const CUtensorMapDataType dt =
+      dtype == MHC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return o.k_major ? make_tmap_2d(m, o.p, dt, 2, k, mn, o.ld * 2, gk::BK, gk::BM,
+                                  CU_TENSOR_MAP_SWIZZLE_128B)
+                   : make_tmap_2d(m, o.p, dt, 2, mn, k, o.ld * 2, 64, gk::BK,
+                                  CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename E, int KIND>
+static int gemm_launch(const Gemm& g, cudaStream_t s) {
+  using namespace gk;
+  constexpr bool dual = KIND == kEpiGated;
+  GemmMaps m;
+  int st;
+  if ((st = operand_map(&m.a, g.a, g.dtype, g.M, g.K))) return st;
+  if ((st = operand_map(&m.b, g.b, g.dtype, g.N, g.K))) return st;
+  m.b2 = m.b; m.a3 = m.a; m.b3 = m.b;
+  if (dual && (st = operand_map(&m.b2, g.b2, g.dtype, g.N, g.K))) return st;
+  if (g.K3 > 0) {
+    if ((st = operand_map(&m.a3, g.a3, g.dtype, g.M, g.K3))) return st;
+    if ((st = operand_map(&m.b3, g.b3, g.dtype, g.N, g.K3))) return st;
+  }
+  GemmWalk w;
+  w.M = g.M; w.N = g.N;
+  w.tiles_m = (int32_t)cdiv(g.M, 2 * BM);
+  w.tiles_n = (int32_t)cdiv(g.N, dual ? BNC : 2 * BNC);
+  w.nk1 = (int32_t)cdiv(g.K, BK);
+  w.nk = w.nk1 + (int32_t)cdiv(g.K3, BK);
+  w.a_k = g.a.k_major; w.b_k = g.b.k_major;
+  w.a3_k = g.a3.k_major; w.b3_k = g.b3.k_major;
+  static bool attr_set[64];
+  int dev = 0;
+  MHC_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    MHC_CUDA_CHECK(cudaFuncSetAttribute((const void*)gemm_kernel<E, KIND>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  const int64_t tiles = (int64_t)w.tiles_m * w.tiles_n;
+  if (tiles > INT32_MAX / 2) return MHC_ERR_INVALID_ARGUMENT;
+  const int clusters = (int)std::min<int64_t>(tiles, sm_count() / 2);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * clusters);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = (!pdl_first_launch() && pdl_enabled()) ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, gemm_kernel<E, KIND>, m, w, g.epi) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return MHC_ERR_CUDA;
+  }
   MHC_LAUNCH_CHECK();
   return MHC_OK;
+}
+
+template <typename E>
+static int gemm_typed(const Gemm& g, cudaStream_t s) {
+  if (g.kind == kEpiGated) return gemm_launch<E, kEpiGated>(g, s);
+  if (g.kind == kEpiGatedBwd) return gemm_launch<E, kEpiGatedBwd>(g, s);
+  return gemm_launch<E, kEpiLinear>(g, s);
 }
 
 int gemm_run(const Gemm& g0, cudaStream_t s) {
   Gemm g = g0;
   g.epi.vec = epi_vec_ok(g);
   return g.dtype == MHC_F16 ? gemm_typed<__half>(g, s) : gemm_typed<__nv_bfloat16>(g, s);
+}
+
+int gemm_device_error() { return read_and_clear_tu_error(); }
+
+// ---------------------------------------------------------------- packed copies
+// Rows of an operand that TMA cannot address (base or row stride off 16 bytes), copied to
+// rows that start on 16-byte boundaries.
+template <int V>  // bytes per access
+__global__ void __launch_bounds__(256)
+    pack_rows_kernel(const char* __restrict__ src, int64_t ls, int64_t rows, int64_t row_bytes,
+                     char* __restrict__ dst, int64_t ld) {
+  pdl_enter();
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < row_bytes;
+         i += (int64_t)gridDim.x * 256 * V) {
+      if constexpr (V == 4)
+        *(uint32_t*)(dst + r * ld + i) = __ldg((const uint32_t*)(src + r * ls + i));
+      else
+        *(uint16_t*)(dst + r * ld + i) = __ldg((const uint16_t*)(src + r * ls + i));
+    }
+}
+
+int pack_rows(const void* src, int64_t ls, int64_t rows, int64_t cols, void* dst, int64_t ld,
+              cudaStream_t s) {
+  const bool four = (reinterpret_cast<uintptr_t>(src) & 3) == 0 && ls % 2 == 0 && cols % 2 == 0;
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv(cols * 2, 256 * (four ? 4 : 2)), 64),
+                  (unsigned)std::min<int64_t>(rows, 16384));
+  if (four)
+    launch(pack_rows_kernel<4>, grid, 256, 0, s, (const char*)src, ls * 2, rows, cols * 2,
+           (char*)dst, ld * 2);
+  else
+    launch(pack_rows_kernel<2>, grid, 256, 0, s, (const char*)src, ls * 2, rows, cols * 2,
+           (char*)dst, ld * 2);
+  MHC_LAUNCH_CHECK();
+  return MHC_OK;
 }
 
 }  // namespace mhc

@@ -50,7 +50,14 @@ struct Gemm {
   EpiParams epi;
 };
 
+// Operands must be aligned (operand_aligned).
 int gemm_run(const Gemm& g, cudaStream_t s);
+
+// Base and rows on 16-byte boundaries, as TMA reads them.
+bool operand_aligned(const Operand& o);
+// Copies (rows, cols) 16-bit elements, rows ls apart, to rows ld apart.
+int pack_rows(const void* src, int64_t ls, int64_t rows, int64_t cols, void* dst, int64_t ld,
+              cudaStream_t s);
 
 // Whether all rows the epilogue touches start on 16-byte boundaries.
 bool epi_vec_ok(const Gemm& g);

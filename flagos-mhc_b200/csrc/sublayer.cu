@@ -1,5 +1,7 @@
 // sublayer.cu -- entry points of the linear layer and the gated feed-forward block: argument
 // checks, workspace layout and the sequence of matrix products (gemm.cuh).
+#include <initializer_list>
+
 #include "gemm.cuh"
 
 namespace mhc {
@@ -92,6 +94,22 @@ struct Carver {
   }
 };
 
+// An operand as the matrix product takes it: itself, or a packed copy in the workspace.
+static int64_t packed_bytes(int64_t rows, int64_t cols) { return rows * pad8(cols) * 2; }
+static int aligned_operand(Operand* o, int64_t rows, int64_t cols, Carver* c, cudaStream_t s) {
+  if (operand_aligned(*o)) return MHC_OK;
+  void* dst = c->take(packed_bytes(rows, cols));
+  const int st = pack_rows(o->p, o->ld, rows, cols, dst, pad8(cols), s);
+  o->p = dst;
+  o->ld = pad8(cols);
+  return st;
+}
+static bool any_unaligned(std::initializer_list<Operand> ops) {
+  for (const Operand& o : ops)
+    if (!operand_aligned(o)) return true;
+  return false;
+}
+
 static int zero(void* p, size_t bytes, cudaStream_t s) {
   if (p && bytes) MHC_CUDA_CHECK(cudaMemsetAsync(p, 0, bytes, s));
   return MHC_OK;
@@ -111,9 +129,13 @@ extern "C" {
 
 size_t mhc_linear_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
                                       int32_t unaligned) {
-  (void)unaligned;
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
-  return 0;
+  Carver c{nullptr};
+  if (unaligned) {
+    c.take(packed_bytes(T, D));  // x
+    c.take(packed_bytes(F, D));  // weight
+  }
+  return c.off;
 }
 
 int mhc_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
@@ -125,26 +147,34 @@ int mhc_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t 
     return MHC_ERR_INVALID_ARGUMENT;
   if (T == 0) return MHC_OK;
   if (!x || !weight || !y) return MHC_ERR_INVALID_ARGUMENT;
-  if (!ws_ok(workspace, workspace_bytes, mhc_linear_fwd_workspace_bytes(T, D, F, dtype, 0)))
-    return MHC_ERR_WORKSPACE;
-  RETURN_IF(check_device());
   Gemm g;
   g.dtype = dtype;
   g.M = T; g.N = F; g.K = D;
   g.a = {x, x_stride, true};
   g.b = {weight, weight_stride, true};
+  if (!ws_ok(workspace, workspace_bytes,
+             mhc_linear_fwd_workspace_bytes(T, D, F, dtype, any_unaligned({g.a, g.b}))))
+    return MHC_ERR_WORKSPACE;
+  RETURN_IF(check_device());
+  const cudaStream_t s = (cudaStream_t)stream;
+  Carver c{(char*)workspace};
+  RETURN_IF(aligned_operand(&g.a, T, D, &c, s));
+  RETURN_IF(aligned_operand(&g.b, F, D, &c, s));
   g.epi.act = act; g.epi.out = y; g.epi.ld_out = F; g.epi.bias = bias; g.epi.z = z;
   g.epi.res = residual; g.epi.ld_res = residual ? residual_stride : 0;
-  return gemm_run(g, (cudaStream_t)stream);
+  return gemm_run(g, s);
 }
 
 size_t mhc_linear_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
                                       int32_t act, int32_t unaligned) {
-  (void)unaligned;
   if (sub_check(T, D, F, dtype, act) != MHC_OK) return 0;
   Carver c{nullptr};
-  if (act != MHC_ACT_NONE) c.take((size_t)T * pad8(F) * 2);
+  if (act != MHC_ACT_NONE || unaligned) c.take(packed_bytes(T, F));  // gz
   c.take((size_t)gz_ranges(T) * F * 4);
+  if (unaligned) {
+    c.take(packed_bytes(T, D));  // x
+    c.take(packed_bytes(F, D));  // weight
+  }
   return c.off;
 }
 
@@ -160,8 +190,11 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   const cudaStream_t s = (cudaStream_t)stream;
   if (T > 0 && (!x || !weight || !grad_y || (act != MHC_ACT_NONE && !z)))
     return MHC_ERR_INVALID_ARGUMENT;
+  Operand ox{x, x_stride, false}, ow{weight, weight_stride, false};
+  const bool gy_packed = act == MHC_ACT_NONE && !operand_aligned({grad_y, grad_y_stride, false});
   if (T > 0 && !ws_ok(workspace, workspace_bytes,
-                      mhc_linear_bwd_workspace_bytes(T, D, F, dtype, act, 0)))
+                      mhc_linear_bwd_workspace_bytes(T, D, F, dtype, act,
+                                                     gy_packed || any_unaligned({ox, ow}))))
     return MHC_ERR_WORKSPACE;
   RETURN_IF(check_device());
   if (T == 0) {
@@ -169,7 +202,8 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
     return zero(grad_bias, (size_t)F * 2, s);
   }
   Carver c{(char*)workspace};
-  void* gzb = act != MHC_ACT_NONE ? c.take((size_t)T * pad8(F) * 2) : nullptr;
+  // without an activation gz is grad_y, copied only where its rows are unaligned
+  void* gzb = act != MHC_ACT_NONE || gy_packed ? c.take(packed_bytes(T, F)) : nullptr;
   float* part = (float*)c.take((size_t)gz_ranges(T) * F * 4);
   if (gzb || grad_bias) {
     const int64_t ld = pad8(F);
@@ -184,16 +218,18 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   Gemm g;
   g.dtype = dtype;
   if (grad_x) {
+    RETURN_IF(aligned_operand(&ow, F, D, &c, s));
     g.M = T; g.N = D; g.K = F;
     g.a = {gz, gzs, true};
-    g.b = {weight, weight_stride, false};
+    g.b = ow;
     g.epi.out = grad_x; g.epi.ld_out = D;
     RETURN_IF(gemm_run(g, s));
   }
   if (grad_weight) {
+    RETURN_IF(aligned_operand(&ox, T, D, &c, s));
     g.M = F; g.N = D; g.K = T;
     g.a = {gz, gzs, false};
-    g.b = {x, x_stride, false};
+    g.b = ox;
     g.epi.out = grad_weight; g.epi.ld_out = D;
     RETURN_IF(gemm_run(g, s));
   }
@@ -202,10 +238,14 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
 
 size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
                                          int32_t unaligned) {
-  (void)unaligned;
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
   Carver c{nullptr};
-  c.take((size_t)T * pad8(F) * 2);  // h
+  c.take(packed_bytes(T, F));  // h
+  if (unaligned) {
+    c.take(packed_bytes(T, D));                              // x
+    for (int i = 0; i < 2; ++i) c.take(packed_bytes(F, D));  // w_gate, w_up
+    c.take(packed_bytes(D, F));                              // w_down
+  }
   return c.off;
 }
 
@@ -220,20 +260,27 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
     return MHC_ERR_INVALID_ARGUMENT;
   if (T == 0) return MHC_OK;
   if (!x || !w_gate || !w_up || !w_down || !y) return MHC_ERR_INVALID_ARGUMENT;
-  if (!ws_ok(workspace, workspace_bytes, mhc_gated_ffn_fwd_workspace_bytes(T, D, F, dtype, 0)))
+  Operand ox{x, x_stride, true}, og{w_gate, w_gate_stride, true}, ou{w_up, w_up_stride, true},
+      od{w_down, w_down_stride, true};
+  if (!ws_ok(workspace, workspace_bytes,
+             mhc_gated_ffn_fwd_workspace_bytes(T, D, F, dtype, any_unaligned({ox, og, ou, od}))))
     return MHC_ERR_WORKSPACE;
   RETURN_IF(check_device());
   const cudaStream_t s = (cudaStream_t)stream;
   Carver c{(char*)workspace};
   const int64_t ldh = pad8(F);
-  void* h = c.take((size_t)T * ldh * 2);
+  void* h = c.take(packed_bytes(T, F));
+  RETURN_IF(aligned_operand(&ox, T, D, &c, s));
+  RETURN_IF(aligned_operand(&og, F, D, &c, s));
+  RETURN_IF(aligned_operand(&ou, F, D, &c, s));
+  RETURN_IF(aligned_operand(&od, D, F, &c, s));
   Gemm g;
   g.kind = kEpiGated;
   g.dtype = dtype;
   g.M = T; g.N = F; g.K = D;
-  g.a = {x, x_stride, true};
-  g.b = {w_gate, w_gate_stride, true};
-  g.b2 = {w_up, w_up_stride, true};
+  g.a = ox;
+  g.b = og;
+  g.b2 = ou;
   g.epi.act = act; g.epi.out = h; g.epi.ld_out = ldh;
   g.epi.gate = gate; g.epi.up = up; g.epi.ld_gu = gate ? gate_up_stride : 0;
   RETURN_IF(gemm_run(g, s));
@@ -241,17 +288,21 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   d.dtype = dtype;
   d.M = T; d.N = D; d.K = F;
   d.a = {h, ldh, true};
-  d.b = {w_down, w_down_stride, true};
+  d.b = od;
   d.epi.out = y; d.epi.ld_out = D;
   return gemm_run(d, s);
 }
 
 size_t mhc_gated_ffn_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
                                          int32_t unaligned) {
-  (void)unaligned;
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
   Carver c{nullptr};
-  for (int i = 0; i < 3; ++i) c.take((size_t)T * pad8(F) * 2);  // gg, gu, h
+  for (int i = 0; i < 3; ++i) c.take(packed_bytes(T, F));  // gg, gu, h
+  if (unaligned) {
+    for (int i = 0; i < 2; ++i) c.take(packed_bytes(T, D));  // x, grad_y
+    for (int i = 0; i < 2; ++i) c.take(packed_bytes(F, D));  // w_gate, w_up
+    c.take(packed_bytes(D, F));                              // w_down
+  }
   return c.off;
 }
 
@@ -269,8 +320,12 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
   const cudaStream_t s = (cudaStream_t)stream;
   if (T > 0 && (!x || !w_gate || !w_up || !w_down || !gate || !up || !grad_y))
     return MHC_ERR_INVALID_ARGUMENT;
-  if (T > 0 && !ws_ok(workspace, workspace_bytes,
-                      mhc_gated_ffn_bwd_workspace_bytes(T, D, F, dtype, 0)))
+  Operand ox{x, x_stride, false}, oy{grad_y, grad_y_stride, true},
+      og{w_gate, w_gate_stride, false}, ou{w_up, w_up_stride, false},
+      od{w_down, w_down_stride, false};
+  if (T > 0 &&
+      !ws_ok(workspace, workspace_bytes,
+             mhc_gated_ffn_bwd_workspace_bytes(T, D, F, dtype, any_unaligned({ox, oy, og, ou, od}))))
     return MHC_ERR_WORKSPACE;
   RETURN_IF(check_device());
   if (T == 0) {
@@ -280,16 +335,18 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
   }
   Carver c{(char*)workspace};
   const int64_t ld = pad8(F);
-  void* gg = c.take((size_t)T * ld * 2);
-  void* gu = c.take((size_t)T * ld * 2);
-  void* h = c.take((size_t)T * ld * 2);
+  void* gg = c.take(packed_bytes(T, F));
+  void* gu = c.take(packed_bytes(T, F));
+  void* h = c.take(packed_bytes(T, F));
+  RETURN_IF(aligned_operand(&oy, T, D, &c, s));
+  RETURN_IF(aligned_operand(&od, D, F, &c, s));
   {
     Gemm g;  // gh = grad_y w_down, then gg, gu and h in its epilogue
     g.kind = kEpiGatedBwd;
     g.dtype = dtype;
     g.M = T; g.N = F; g.K = D;
-    g.a = {grad_y, grad_y_stride, true};
-    g.b = {w_down, w_down_stride, false};
+    g.a = oy;
+    g.b = od;
     g.epi.act = act;
     g.epi.gate = const_cast<void*>(gate); g.epi.up = const_cast<void*>(up);
     g.epi.ld_gu = gate_up_stride;
@@ -300,19 +357,22 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
   Gemm g;
   g.dtype = dtype;
   if (grad_x) {
+    RETURN_IF(aligned_operand(&og, F, D, &c, s));
+    RETURN_IF(aligned_operand(&ou, F, D, &c, s));
     g.M = T; g.N = D; g.K = F;
     g.a = {gg, ld, true};
-    g.b = {w_gate, w_gate_stride, false};
+    g.b = og;
     g.a3 = {gu, ld, true};
-    g.b3 = {w_up, w_up_stride, false};
+    g.b3 = ou;
     g.K3 = F;
     g.epi.out = grad_x; g.epi.ld_out = D;
     RETURN_IF(gemm_run(g, s));
     g.K3 = 0;
   }
+  if (grad_w_gate || grad_w_up) RETURN_IF(aligned_operand(&ox, T, D, &c, s));
   g.K = T;
   g.M = F; g.N = D;
-  g.b = {x, x_stride, false};
+  g.b = ox;
   g.epi.ld_out = D;
   if (grad_w_gate) {
     g.a = {gg, ld, false};
@@ -326,7 +386,7 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
   }
   if (grad_w_down) {
     g.M = D; g.N = F;
-    g.a = {grad_y, grad_y_stride, false};
+    g.a = {oy.p, oy.ld, false};
     g.b = {h, ld, false};
     g.epi.out = grad_w_down; g.epi.ld_out = F;
     RETURN_IF(gemm_run(g, s));
