@@ -32,6 +32,7 @@ int post_mix_run(const void* x, const float* h_res, const void* h_out, const flo
                  float* premix, int32_t layers, void* ws, cudaStream_t s);
 int tc_host_device_error();
 int gemm_device_error();
+int layer_norm_device_error();
 
 static std::atomic<unsigned long long> g_launches{0};
 void note_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
@@ -76,6 +77,9 @@ int check_device() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return MHC_ERR_CUDA;
   if (dev < 0 || dev >= 64) return MHC_ERR_DEVICE;
+  // A thread that has made no runtime call yet (autograd's, for one) has no current context,
+  // and the tensor-map encoder, a driver call, fails there: this binds the device's.
+  if (cudaSetDevice(dev) != cudaSuccess) return MHC_ERR_CUDA;
   if (g_arch_ok[dev] == 0) {
     int major = 0, minor = 0;
     if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
@@ -148,7 +152,8 @@ int mhc_device_status(void) {
   const int f = post_mix_device_error();
   const int g = pre_bwd_tc32_device_error();
   const int h = gemm_device_error();
-  const int all[8] = {a, b, c, d, e, f, g, h};
+  const int i = layer_norm_device_error();
+  const int all[9] = {a, b, c, d, e, f, g, h, i};
   for (int v : all)
     if (v != MHC_OK) return v;
   return MHC_OK;

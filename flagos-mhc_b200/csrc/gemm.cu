@@ -21,13 +21,16 @@ namespace gk {
 constexpr int BM = 128;          // rows of A per CTA (256 per cluster)
 constexpr int BNC = 128;         // rows of B per CTA (256 per cluster)
 constexpr int BK = 64;
-constexpr int STAGES = 6;
 constexpr int A_BYTES = BM * BK * 2, B_BYTES = BNC * BK * 2;
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
-constexpr int SMEM = STAGES * STAGE_BYTES + 1024;  // and room to align
-constexpr int GROUP_M = 8;       // row tiles that walk the column tiles together
+constexpr int GROUP_ROWS = 2048;  // rows of tiles that walk the column tiles together
+// MT accumulators of 256 rows to a tile
+template <int MT> struct Ring {
+  static constexpr int STAGES = MT == 1 ? 6 : 4;
+  static constexpr int STAGE_BYTES = MT * A_BYTES + B_BYTES;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;  // and room to align
+};
 }  // namespace gk
 
 struct GemmMaps {
@@ -57,7 +60,7 @@ __device__ __forceinline__ uint32_t leader_addr(const void* p) {
   return r;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // a third of a second at least; the longest healthy wait is one tile's products
 constexpr uint32_t kSpin = 1u << 24;
@@ -66,7 +69,7 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, vol
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(tc::smem_u32(bar)), "r"(parity)
@@ -118,22 +121,26 @@ __device__ __forceinline__ void ld32(uint32_t taddr, float* v) {
 }
 }  // namespace tc2
 
-// tile index -> tile row and column: GROUP_M row tiles walk all column tiles together, so the
+// tile index -> tile row and column: GROUP row tiles walk all column tiles together, so the
 // tiles in flight share their operands in L2
+template <int MT>
 __device__ __forceinline__ void tile_at(const GemmWalk& w, int32_t i, int32_t& mt, int32_t& nt) {
-  const int32_t per = gk::GROUP_M * w.tiles_n;
+  constexpr int32_t GROUP = gk::GROUP_ROWS / (256 * MT);
+  const int32_t per = GROUP * w.tiles_n;
   const int32_t g = i / per, rest = i - g * per;
-  const int32_t rows = min(gk::GROUP_M, w.tiles_m - g * gk::GROUP_M);
+  const int32_t rows = min(GROUP, w.tiles_m - g * GROUP);
   nt = rest / rows;
-  mt = g * gk::GROUP_M + rest - nt * rows;
+  mt = g * GROUP + rest - nt * rows;
 }
 
-template <typename E, int KIND>
+template <typename E, int KIND, int MT>
 __global__ void __launch_bounds__(gk::THREADS, 1)
     gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmWalk w,
                 const __grid_constant__ EpiParams epi) {
   using namespace gk;
   constexpr bool dual = KIND == kEpiGated;
+  constexpr int STAGES = Ring<MT>::STAGES, STAGE_BYTES = Ring<MT>::STAGE_BYTES;
+  constexpr int ROWS = 256 * MT;  // of a tile
   extern __shared__ char smem_raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                        ~uintptr_t(1023));
@@ -151,7 +158,7 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&tfull[i], 1);
-      tc::mbar_init(&tempty[i], 2 * EPI_WARPS);
+      tc::mbar_init(&tempty[i], 2 * EPI_WARPS / MT);
     }
     tc::mbar_init(&tdone, 1);
     abort_word = 0;
@@ -181,8 +188,8 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
       bool ok = true;
       for (int32_t i = first; i < tiles && ok; i += step) {
         int32_t mt, nt;
-        tile_at(w, i, mt, nt);
-        const int32_t m0 = mt * 2 * BM + (int32_t)rank * BM;
+        tile_at<MT>(w, i, mt, nt);
+        const int32_t m0 = mt * ROWS + (int32_t)rank * BM;
         const int32_t n0 = dual ? nt * BNC : nt * 2 * BNC + (int32_t)rank * BNC;
         for (int32_t kb = 0; kb < w.nk; ++kb, ++it) {
           const uint32_t s = it % STAGES;
@@ -192,16 +199,21 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
           }
           if (leader) tc::mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
           const uint32_t bar = tc2::leader_addr(&full[s]);
-          const uint32_t sa = tc::smem_u32(smem + s * STAGE_BYTES), sb = sa + A_BYTES;
+          const uint32_t sa = tc::smem_u32(smem + s * STAGE_BYTES), sb = sa + MT * A_BYTES;
           const bool second = kb >= w.nk1;
           const int32_t k0 = (second ? kb - w.nk1 : kb) * BK;
           const CUtensorMap* ma = second ? &maps.a3 : &maps.a;
           const CUtensorMap* mb = second ? &maps.b3 : (dual && rank) ? &maps.b2 : &maps.b;
-          if (second ? w.a3_k : w.a_k) {
-            tc2::load_2d(sa, ma, bar, k0, m0);
-          } else {
-            tc2::load_2d(sa, ma, bar, m0, k0);
-            tc2::load_2d(sa + A_BYTES / 2, ma, bar, m0 + 64, k0);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const uint32_t dst = sa + m * A_BYTES;
+            const int32_t r0 = m0 + m * 256;
+            if (second ? w.a3_k : w.a_k) {
+              tc2::load_2d(dst, ma, bar, k0, r0);
+            } else {
+              tc2::load_2d(dst, ma, bar, r0, k0);
+              tc2::load_2d(dst + A_BYTES / 2, ma, bar, r0 + 64, k0);
+            }
           }
           if (second ? w.b3_k : w.b_k) {
             tc2::load_2d(sb, mb, bar, k0, n0);
@@ -222,10 +234,11 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
         uint32_t it = 0, j = 0;
         bool ok = true;
         for (int32_t i = first; i < tiles && ok; i += step, ++j) {
-          const uint32_t buf = j & 1;
-          if (!tc2::wait_cluster(&tempty[buf], ((j >> 1) & 1) ^ 1, abort_flag)) break;
+          // MT = 1: tiles take the two accumulators in turn; MT = 2: each tile takes both
+          const uint32_t buf = MT == 1 ? j & 1 : 0, ph = MT == 1 ? (j >> 1) & 1 : j & 1;
+          if (!tc2::wait_cluster(&tempty[buf], ph ^ 1, abort_flag)) break;
+          if (MT == 2 && !tc2::wait_cluster(&tempty[1], ph ^ 1, abort_flag)) break;
           tc::tc_fence_after();
-          const uint32_t d = tmem + buf * 256;
           for (int32_t kb = 0; kb < w.nk; ++kb, ++it) {
             const uint32_t s = it % STAGES;
             if (!tc2::wait_cluster(&full[s], (it / STAGES) & 1, abort_flag)) {
@@ -236,18 +249,24 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
             const bool second = kb >= w.nk1;
             const bool ak = second ? w.a3_k : w.a_k, bk = second ? w.b3_k : w.b_k;
             const uint32_t sa = tc::smem_u32(smem + s * STAGE_BYTES);
-            const uint64_t da = tc::smem_desc(sa, ak ? 16 : A_BYTES / 2, 1024, tc::kSwizzle128);
-            const uint64_t db =
-                tc::smem_desc(sa + A_BYTES, bk ? 16 : B_BYTES / 2, 1024, tc::kSwizzle128);
+            const uint64_t db = tc::smem_desc(sa + MT * A_BYTES, bk ? 16 : B_BYTES / 2, 1024,
+                                              tc::kSwizzle128);
             const uint32_t stepa = ak ? 2 : 128, stepb = bk ? 2 : 128;
+            const uint32_t idesc = second ? idesc2 : idesc1;
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              tc2::mma(d, da + k * stepa, db + k * stepb, second ? idesc2 : idesc1,
-                       (kb != 0 || k != 0) ? 1u : 0u);
+            for (int m = 0; m < MT; ++m) {
+              const uint64_t da = tc::smem_desc(sa + m * A_BYTES, ak ? 16 : A_BYTES / 2, 1024,
+                                                tc::kSwizzle128);
+              const uint32_t d = tmem + (buf + m) * 256;
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k)
+                tc2::mma(d, da + k * stepa, db + k * stepb, idesc, (kb != 0 || k != 0) ? 1u : 0u);
+              if (MT == 2 && kb + 1 == w.nk) tc2::commit_both(&tfull[m]);
+            }
             tc2::commit_both(&empty[s]);
           }
           if (!ok) break;
-          tc2::commit_both(&tfull[buf]);
+          if (MT == 1) tc2::commit_both(&tfull[buf]);
         }
         tc2::commit_both(&tdone);  // every MMA has completed before TMEM is freed
       }
@@ -256,19 +275,22 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
     }
   } else {
     // ---------------------------------------------------------------- epilogue
-    constexpr int COLS = dual ? BNC / 2 : BNC;  // output columns per warp
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t tq = tmem + ((uint32_t)(q * 32) << 16) + half * COLS;
+    // eight warps, four lane quarters: the pair of a quarter splits the columns of the one
+    // accumulator, or takes an accumulator each
+    constexpr int COLS = (dual ? BNC : 2 * BNC) / (MT == 1 ? 2 : 1);  // output columns per warp
+    const int q = warp & 3, pair = (warp - 2) >> 2;
+    const int col_off = MT == 1 ? pair * COLS : 0;
+    const uint32_t tq = tmem + ((uint32_t)(q * 32) << 16) + col_off;
     uint32_t j = 0;
     for (int32_t i = first; i < tiles; i += step, ++j) {
       int32_t mt, nt;
-      tile_at(w, i, mt, nt);
-      const uint32_t buf = j & 1;
-      const bool got = tc2::wait_cluster(&tfull[buf], (j >> 1) & 1, abort_flag);
+      tile_at<MT>(w, i, mt, nt);
+      const uint32_t buf = MT == 1 ? j & 1 : pair, ph = MT == 1 ? (j >> 1) & 1 : j & 1;
+      const bool got = tc2::wait_cluster(&tfull[buf], ph, abort_flag);
       if (!__all_sync(0xffffffffu, got)) break;
       tc::tc_fence_after();
-      const int64_t row = (int64_t)mt * 2 * BM + rank * BM + q * 32 + lane;
-      const int64_t col0 = (int64_t)nt * (dual ? BNC : 2 * BNC) + half * COLS;
+      const int64_t row = (int64_t)mt * ROWS + (MT == 1 ? 0 : pair * 256) + rank * BM + q * 32 + lane;
+      const int64_t col0 = (int64_t)nt * (dual ? BNC : 2 * BNC) + col_off;
 #pragma unroll 1
       for (int c = 0; c < COLS; c += 32) {
         __syncwarp();  // rows past M skip the epilogue below
@@ -316,7 +338,7 @@ static int operand_map(CUtensorMap* m, const Operand& o, int32_t dtype, int64_t 
                                   CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename E, int KIND>
+template <typename E, int KIND, int MT>
 static int gemm_launch(const Gemm& g, cudaStream_t s) {
   using namespace gk;
   constexpr bool dual = KIND == kEpiGated;
@@ -332,18 +354,19 @@ static int gemm_launch(const Gemm& g, cudaStream_t s) {
   }
   GemmWalk w;
   w.M = g.M; w.N = g.N;
-  w.tiles_m = (int32_t)cdiv(g.M, 2 * BM);
+  w.tiles_m = (int32_t)cdiv(g.M, 256 * MT);
   w.tiles_n = (int32_t)cdiv(g.N, dual ? BNC : 2 * BNC);
   w.nk1 = (int32_t)cdiv(g.K, BK);
   w.nk = w.nk1 + (int32_t)cdiv(g.K3, BK);
   w.a_k = g.a.k_major; w.b_k = g.b.k_major;
   w.a3_k = g.a3.k_major; w.b3_k = g.b3.k_major;
+  constexpr int smem = Ring<MT>::SMEM;
   static bool attr_set[64];
   int dev = 0;
   MHC_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    MHC_CUDA_CHECK(cudaFuncSetAttribute((const void*)gemm_kernel<E, KIND>,
-                                        cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    MHC_CUDA_CHECK(cudaFuncSetAttribute((const void*)gemm_kernel<E, KIND, MT>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   const int64_t tiles = (int64_t)w.tiles_m * w.tiles_n;
@@ -359,11 +382,11 @@ static int gemm_launch(const Gemm& g, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * clusters);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = (!pdl_first_launch() && pdl_enabled()) ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, gemm_kernel<E, KIND>, m, w, g.epi) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, gemm_kernel<E, KIND, MT>, m, w, g.epi) != cudaSuccess) {
     (void)cudaGetLastError();
     return MHC_ERR_CUDA;
   }
@@ -373,9 +396,13 @@ static int gemm_launch(const Gemm& g, cudaStream_t s) {
 
 template <typename E>
 static int gemm_typed(const Gemm& g, cudaStream_t s) {
-  if (g.kind == kEpiGated) return gemm_launch<E, kEpiGated>(g, s);
-  if (g.kind == kEpiGatedBwd) return gemm_launch<E, kEpiGatedBwd>(g, s);
-  return gemm_launch<E, kEpiLinear>(g, s);
+  static const int force = getenv("MT") ? atoi(getenv("MT")) : 1;
+  if (g.kind == kEpiGated)
+    return force == 2 ? gemm_launch<E, kEpiGated, 2>(g, s) : gemm_launch<E, kEpiGated, 1>(g, s);
+  if (g.kind == kEpiGatedBwd)
+    return force == 2 ? gemm_launch<E, kEpiGatedBwd, 2>(g, s)
+                      : gemm_launch<E, kEpiGatedBwd, 1>(g, s);
+  return force == 2 ? gemm_launch<E, kEpiLinear, 2>(g, s) : gemm_launch<E, kEpiLinear, 1>(g, s);
 }
 
 int gemm_run(const Gemm& g0, cudaStream_t s) {
