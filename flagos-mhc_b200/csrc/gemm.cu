@@ -41,6 +41,9 @@ struct GemmWalk {
   int64_t M, N;                       // of the output
   int32_t tiles_m, tiles_n, nk1, nk;  // K blocks of the first segment, of both
   int32_t a_k, b_k, a3_k, b3_k;       // operands that are K-major
+  int32_t splits;                     // ranges of K, each a unit of work of its own
+  float* part;                        // splits > 1: [splits][planes][M][ldp] partial products
+  int64_t ldp;
 };
 
 namespace tc2 {
@@ -123,14 +126,25 @@ __device__ __forceinline__ void ld32(uint32_t taddr, float* v) {
 
 // tile index -> tile row and column: GROUP row tiles walk all column tiles together, so the
 // tiles in flight share their operands in L2
+// Unit i is tile i % tiles of K range i / tiles.
+struct Unit {
+  int32_t mt, nt, split, kb0, kb1;
+};
 template <int MT>
-__device__ __forceinline__ void tile_at(const GemmWalk& w, int32_t i, int32_t& mt, int32_t& nt) {
+__device__ __forceinline__ Unit unit_at(const GemmWalk& w, int32_t u) {
+  Unit r;
+  const int32_t tiles = w.tiles_m * w.tiles_n;
+  r.split = u / tiles;
+  const int32_t i = u - r.split * tiles;
+  r.kb0 = (int32_t)((int64_t)w.nk * r.split / w.splits);
+  r.kb1 = (int32_t)((int64_t)w.nk * (r.split + 1) / w.splits);
   constexpr int32_t GROUP = gk::GROUP_ROWS / (256 * MT);
   const int32_t per = GROUP * w.tiles_n;
   const int32_t g = i / per, rest = i - g * per;
   const int32_t rows = min(GROUP, w.tiles_m - g * GROUP);
-  nt = rest / rows;
-  mt = g * GROUP + rest - nt * rows;
+  r.nt = rest / rows;
+  r.mt = g * GROUP + rest - r.nt * rows;
+  return r;
 }
 
 template <typename E, int KIND, int MT>
@@ -179,19 +193,18 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
   const uint32_t tmem = *(volatile uint32_t*)&tmem_slot;
   pdl_enter();
 
-  const int32_t tiles = w.tiles_m * w.tiles_n;
+  const int32_t units = w.tiles_m * w.tiles_n * w.splits;
   const int32_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int32_t i = first; i < tiles && ok; i += step) {
-        int32_t mt, nt;
-        tile_at<MT>(w, i, mt, nt);
-        const int32_t m0 = mt * ROWS + (int32_t)rank * BM;
-        const int32_t n0 = dual ? nt * BNC : nt * 2 * BNC + (int32_t)rank * BNC;
-        for (int32_t kb = 0; kb < w.nk; ++kb, ++it) {
+      for (int32_t i = first; i < units && ok; i += step) {
+        const Unit u = unit_at<MT>(w, i);
+        const int32_t m0 = u.mt * ROWS + (int32_t)rank * BM;
+        const int32_t n0 = dual ? u.nt * BNC : u.nt * 2 * BNC + (int32_t)rank * BNC;
+        for (int32_t kb = u.kb0; kb < u.kb1; ++kb, ++it) {
           const uint32_t s = it % STAGES;
           if (!tc2::wait_cluster(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag)) {
             ok = false;
@@ -233,13 +246,14 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
         const uint32_t idesc2 = tc::idesc_16<E>(256, 256, !w.a3_k, !w.b3_k);
         uint32_t it = 0, j = 0;
         bool ok = true;
-        for (int32_t i = first; i < tiles && ok; i += step, ++j) {
+        for (int32_t i = first; i < units && ok; i += step, ++j) {
+          const Unit u = unit_at<MT>(w, i);
           // MT = 1: tiles take the two accumulators in turn; MT = 2: each tile takes both
           const uint32_t buf = MT == 1 ? j & 1 : 0, ph = MT == 1 ? (j >> 1) & 1 : j & 1;
           if (!tc2::wait_cluster(&tempty[buf], ph ^ 1, abort_flag)) break;
           if (MT == 2 && !tc2::wait_cluster(&tempty[1], ph ^ 1, abort_flag)) break;
           tc::tc_fence_after();
-          for (int32_t kb = 0; kb < w.nk; ++kb, ++it) {
+          for (int32_t kb = u.kb0; kb < u.kb1; ++kb, ++it) {
             const uint32_t s = it % STAGES;
             if (!tc2::wait_cluster(&full[s], (it / STAGES) & 1, abort_flag)) {
               ok = false;
@@ -260,8 +274,8 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
               const uint32_t d = tmem + (buf + m) * 256;
 #pragma unroll
               for (int k = 0; k < BK / 16; ++k)
-                tc2::mma(d, da + k * stepa, db + k * stepb, idesc, (kb != 0 || k != 0) ? 1u : 0u);
-              if (MT == 2 && kb + 1 == w.nk) tc2::commit_both(&tfull[m]);
+                tc2::mma(d, da + k * stepa, db + k * stepb, idesc, (kb != u.kb0 || k != 0) ? 1u : 0u);
+              if (MT == 2 && kb + 1 == u.kb1) tc2::commit_both(&tfull[m]);
             }
             tc2::commit_both(&empty[s]);
           }
@@ -282,15 +296,14 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
     const int col_off = MT == 1 ? pair * COLS : 0;
     const uint32_t tq = tmem + ((uint32_t)(q * 32) << 16) + col_off;
     uint32_t j = 0;
-    for (int32_t i = first; i < tiles; i += step, ++j) {
-      int32_t mt, nt;
-      tile_at<MT>(w, i, mt, nt);
+    for (int32_t i = first; i < units; i += step, ++j) {
+      const Unit u = unit_at<MT>(w, i);
       const uint32_t buf = MT == 1 ? j & 1 : pair, ph = MT == 1 ? (j >> 1) & 1 : j & 1;
       const bool got = tc2::wait_cluster(&tfull[buf], ph, abort_flag);
       if (!__all_sync(0xffffffffu, got)) break;
       tc::tc_fence_after();
-      const int64_t row = (int64_t)mt * ROWS + (MT == 1 ? 0 : pair * 256) + rank * BM + q * 32 + lane;
-      const int64_t col0 = (int64_t)nt * (dual ? BNC : 2 * BNC) + col_off;
+      const int64_t row = (int64_t)u.mt * ROWS + (MT == 1 ? 0 : pair * 256) + rank * BM + q * 32 + lane;
+      const int64_t col0 = (int64_t)u.nt * (dual ? BNC : 2 * BNC) + col_off;
 #pragma unroll 1
       for (int c = 0; c < COLS; c += 32) {
         __syncwarp();  // rows past M skip the epilogue below
@@ -304,8 +317,20 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
           if (lane == 0) tc2::arrive_cluster(tc2::leader_addr(&tempty[buf]));
         }
         const int64_t left = w.N - (col0 + c);
-        if (row < w.M && left > 0)
-          epi_chunk<E, KIND, 32>(epi, row, col0 + c, left < 32 ? (int)left : 32, acc, acc2);
+        if (row < w.M && left > 0) {
+          if (w.splits == 1) {
+            epi_chunk<E, KIND, 32>(epi, row, col0 + c, left < 32 ? (int)left : 32, acc, acc2);
+          } else {  // ldp is N rounded up to 32
+            float* d = w.part + ((int64_t)u.split * (dual ? 2 : 1) * w.M + row) * w.ldp + col0 + c;
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(d + k) = *reinterpret_cast<float4*>(acc + k);
+            if constexpr (dual) {
+              d += w.M * w.ldp;
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(d + k) = *reinterpret_cast<float4*>(acc2 + k);
+            }
+          }
+        }
       }
     }
   }
@@ -318,6 +343,74 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
     tc::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
+}
+
+// Sums the K ranges' partial products in order and runs the epilogue: 8 columns to a thread.
+template <typename E, int KIND>
+__global__ void __launch_bounds__(256)
+    gemm_finish_kernel(const float* __restrict__ part, int splits, int64_t M, int64_t N,
+                       int64_t ldp, const __grid_constant__ EpiParams epi) {
+  pdl_enter();
+  constexpr int PL = KIND == kEpiGated ? 2 : 1;
+  const int64_t cols = ldp / 8, n = M * cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / cols, col = (i - row * cols) * 8;
+    if (col >= N) continue;
+    float acc[PL][8] = {};
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+      const float* d = part + ((int64_t)p * M + row) * ldp + col;
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s, d += PL * M * ldp) {
+        const float4 a = *reinterpret_cast<const float4*>(d);
+        const float4 b = *reinterpret_cast<const float4*>(d + 4);
+        acc[p][0] += a.x; acc[p][1] += a.y; acc[p][2] += a.z; acc[p][3] += a.w;
+        acc[p][4] += b.x; acc[p][5] += b.y; acc[p][6] += b.z; acc[p][7] += b.w;
+      }
+    }
+    epi_chunk<E, KIND, 8>(epi, row, col, N - col < 8 ? (int)(N - col) : 8, acc[0], acc[PL - 1]);
+  }
+}
+
+// How a product is cut: MT accumulators of 256 rows to a tile, `splits` ranges of K.
+struct GemmPlan {
+  int mt, splits;
+};
+static int64_t k_blocks(const Gemm& g) { return cdiv(g.K, gk::BK) + cdiv(g.K3, gk::BK); }
+static int64_t part_ld(const Gemm& g) { return cdiv(g.N, 32) * 32; }
+
+// The cut whose estimated time is least.  Measured on full grids: 0.50 us to a K block of a
+// 256-row tile, 0.86 us of a 512-row one (which reads B half as often for its work, and whose
+// epilogue, with no accumulators left for the next tile, stands alone: 2 us, 3 us with a gate,
+// 20 us with the gate's backward).  A cut in K writes and reads fp32 partials (at 4 TB/s) and
+// takes another launch (3 us).
+static GemmPlan gemm_plan(const Gemm& g) {
+  const bool dual = g.kind == kEpiGated;
+  const int64_t nk = k_blocks(g), clusters = sm_count() / 2;
+  const int64_t tn = cdiv(g.N, dual ? gk::BNC : 2 * gk::BNC);
+  const double plane = (double)g.M * (double)part_ld(g) * (dual ? 2 : 1);
+  GemmPlan best{1, 1};
+  double best_us = 1e30;
+  for (int mt = 1; mt <= 2; ++mt) {
+    if (mt == 2 && g.M <= 256) break;
+    const int64_t tiles = cdiv(g.M, 256 * mt) * tn;
+    const double per_k = mt == 1 ? 0.50 : 0.86;
+    const double tail = mt == 1 ? 1.0 : g.kind == kEpiLinear ? 2.0 : dual ? 3.0 : 20.0;
+    for (int sp = 1; sp <= 16; ++sp) {
+      if (sp > 1 && (nk < 4 * sp || plane * sp * 4 > 1e9)) break;
+      const double waves = (double)cdiv(tiles * sp, clusters);
+      double us = waves * ((double)cdiv(nk, sp) * per_k + tail);
+      if (sp > 1) us += 3.0 + plane * sp * 8 / 4e6;
+      if (us < best_us) best_us = us, best = {mt, sp};
+    }
+  }
+  return best;
+}
+
+size_t gemm_ws_bytes(const Gemm& g) {
+  const GemmPlan p = gemm_plan(g);
+  if (p.splits == 1) return 0;
+  return align_up((size_t)p.splits * (g.kind == kEpiGated ? 2 : 1) * g.M * part_ld(g) * 4);
 }
 
 bool epi_vec_ok(const Gemm& g) {
@@ -339,7 +432,7 @@ static int operand_map(CUtensorMap* m, const Operand& o, int32_t dtype, int64_t 
 }
 
 template <typename E, int KIND, int MT>
-static int gemm_launch(const Gemm& g, cudaStream_t s) {
+static int gemm_launch(const Gemm& g, int splits, float* part, cudaStream_t s) {
   using namespace gk;
   constexpr bool dual = KIND == kEpiGated;
   GemmMaps m;
@@ -360,6 +453,9 @@ static int gemm_launch(const Gemm& g, cudaStream_t s) {
   w.nk = w.nk1 + (int32_t)cdiv(g.K3, BK);
   w.a_k = g.a.k_major; w.b_k = g.b.k_major;
   w.a3_k = g.a3.k_major; w.b3_k = g.b3.k_major;
+  w.splits = splits;
+  w.part = part;
+  w.ldp = part_ld(g);
   constexpr int smem = Ring<MT>::SMEM;
   static bool attr_set[64];
   int dev = 0;
@@ -369,9 +465,9 @@ static int gemm_launch(const Gemm& g, cudaStream_t s) {
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  const int64_t tiles = (int64_t)w.tiles_m * w.tiles_n;
-  if (tiles > INT32_MAX / 2) return MHC_ERR_INVALID_ARGUMENT;
-  const int clusters = (int)std::min<int64_t>(tiles, sm_count() / 2);
+  const int64_t units = (int64_t)w.tiles_m * w.tiles_n * splits;
+  if (units > INT32_MAX / 2) return MHC_ERR_INVALID_ARGUMENT;
+  const int clusters = (int)std::min<int64_t>(units, sm_count() / 2);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -394,21 +490,31 @@ static int gemm_launch(const Gemm& g, cudaStream_t s) {
   return MHC_OK;
 }
 
-template <typename E>
-static int gemm_typed(const Gemm& g, cudaStream_t s) {
-  static const int force = getenv("MT") ? atoi(getenv("MT")) : 1;
-  if (g.kind == kEpiGated)
-    return force == 2 ? gemm_launch<E, kEpiGated, 2>(g, s) : gemm_launch<E, kEpiGated, 1>(g, s);
-  if (g.kind == kEpiGatedBwd)
-    return force == 2 ? gemm_launch<E, kEpiGatedBwd, 2>(g, s)
-                      : gemm_launch<E, kEpiGatedBwd, 1>(g, s);
-  return force == 2 ? gemm_launch<E, kEpiLinear, 2>(g, s) : gemm_launch<E, kEpiLinear, 1>(g, s);
+template <typename E, int KIND>
+static int gemm_kind(const Gemm& g, void* ws, cudaStream_t s) {
+  const GemmPlan p = gemm_plan(g);
+  float* part = p.splits > 1 ? (float*)ws : nullptr;
+  const int st = p.mt == 2 ? gemm_launch<E, KIND, 2>(g, p.splits, part, s)
+                           : gemm_launch<E, KIND, 1>(g, p.splits, part, s);
+  if (st != MHC_OK || !part) return st;
+  const int64_t n = g.M * (part_ld(g) / 8);
+  launch(gemm_finish_kernel<E, KIND>, (unsigned)std::min<int64_t>(cdiv(n, 256), 8 * sm_count()),
+         256, 0, s, (const float*)part, p.splits, g.M, g.N, part_ld(g), g.epi);
+  MHC_LAUNCH_CHECK();
+  return MHC_OK;
 }
 
-int gemm_run(const Gemm& g0, cudaStream_t s) {
+template <typename E>
+static int gemm_typed(const Gemm& g, void* ws, cudaStream_t s) {
+  if (g.kind == kEpiGated) return gemm_kind<E, kEpiGated>(g, ws, s);
+  if (g.kind == kEpiGatedBwd) return gemm_kind<E, kEpiGatedBwd>(g, ws, s);
+  return gemm_kind<E, kEpiLinear>(g, ws, s);
+}
+
+int gemm_run(const Gemm& g0, void* ws, cudaStream_t s) {
   Gemm g = g0;
   g.epi.vec = epi_vec_ok(g);
-  return g.dtype == MHC_F16 ? gemm_typed<__half>(g, s) : gemm_typed<__nv_bfloat16>(g, s);
+  return g.dtype == MHC_F16 ? gemm_typed<__half>(g, ws, s) : gemm_typed<__nv_bfloat16>(g, ws, s);
 }
 
 int gemm_device_error() { return read_and_clear_tu_error(); }

@@ -50,8 +50,10 @@ struct Gemm {
   EpiParams epi;
 };
 
-// Operands must be aligned (operand_aligned).
-int gemm_run(const Gemm& g, cudaStream_t s);
+// Operands must be aligned (operand_aligned).  ws: gemm_ws_bytes, which goes by the kind and the
+// sizes alone.
+size_t gemm_ws_bytes(const Gemm& g);
+int gemm_run(const Gemm& g, void* ws, cudaStream_t s);
 
 // Base and rows on 16-byte boundaries, as TMA reads them.
 bool operand_aligned(const Operand& o);

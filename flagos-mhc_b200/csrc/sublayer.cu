@@ -1,5 +1,6 @@
 // sublayer.cu -- entry points of the linear layer and the gated feed-forward block: argument
 // checks, workspace layout and the sequence of matrix products (gemm.cuh).
+#include <algorithm>
 #include <initializer_list>
 
 #include "gemm.cuh"
@@ -104,6 +105,32 @@ static int aligned_operand(Operand* o, int64_t rows, int64_t cols, Carver* c, cu
   o->ld = pad8(cols);
   return st;
 }
+// Room for the partial products of the largest of these products (they run one by one).
+static Gemm product(int kind, int64_t M, int64_t N, int64_t K, int64_t K3 = 0) {
+  Gemm g;
+  g.kind = kind;
+  g.M = M; g.N = N; g.K = K; g.K3 = K3;
+  return g;
+}
+static size_t gemm_room(std::initializer_list<Gemm> gs) {
+  size_t n = 0;
+  for (const Gemm& g : gs) n = std::max(n, gemm_ws_bytes(g));
+  return n;
+}
+static size_t linear_fwd_room(int64_t T, int64_t D, int64_t F) {
+  return T == 0 ? 0 : gemm_room({product(kEpiLinear, T, F, D)});
+}
+static size_t linear_bwd_room(int64_t T, int64_t D, int64_t F) {
+  return T == 0 ? 0 : gemm_room({product(kEpiLinear, T, D, F), product(kEpiLinear, F, D, T)});
+}
+static size_t ffn_fwd_room(int64_t T, int64_t D, int64_t F) {
+  return T == 0 ? 0 : gemm_room({product(kEpiGated, T, F, D), product(kEpiLinear, T, D, F)});
+}
+static size_t ffn_bwd_room(int64_t T, int64_t D, int64_t F) {
+  return T == 0 ? 0 : gemm_room({product(kEpiGatedBwd, T, F, D), product(kEpiLinear, T, D, F, F),
+                                 product(kEpiLinear, F, D, T), product(kEpiLinear, D, F, T)});
+}
+
 static bool any_unaligned(std::initializer_list<Operand> ops) {
   for (const Operand& o : ops)
     if (!operand_aligned(o)) return true;
@@ -131,6 +158,7 @@ size_t mhc_linear_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t d
                                       int32_t unaligned) {
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
   Carver c{nullptr};
+  c.take(linear_fwd_room(T, D, F));
   if (unaligned) {
     c.take(packed_bytes(T, D));  // x
     c.take(packed_bytes(F, D));  // weight
@@ -158,11 +186,12 @@ int mhc_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   RETURN_IF(check_device());
   const cudaStream_t s = (cudaStream_t)stream;
   Carver c{(char*)workspace};
+  void* room = c.take(linear_fwd_room(T, D, F));
   RETURN_IF(aligned_operand(&g.a, T, D, &c, s));
   RETURN_IF(aligned_operand(&g.b, F, D, &c, s));
   g.epi.act = act; g.epi.out = y; g.epi.ld_out = F; g.epi.bias = bias; g.epi.z = z;
   g.epi.res = residual; g.epi.ld_res = residual ? residual_stride : 0;
-  return gemm_run(g, s);
+  return gemm_run(g, room, s);
 }
 
 size_t mhc_linear_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
@@ -171,6 +200,7 @@ size_t mhc_linear_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t d
   Carver c{nullptr};
   if (act != MHC_ACT_NONE || unaligned) c.take(packed_bytes(T, F));  // gz
   c.take((size_t)gz_ranges(T) * F * 4);
+  c.take(linear_bwd_room(T, D, F));
   if (unaligned) {
     c.take(packed_bytes(T, D));  // x
     c.take(packed_bytes(F, D));  // weight
@@ -205,6 +235,7 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   // without an activation gz is grad_y, copied only where its rows are unaligned
   void* gzb = act != MHC_ACT_NONE || gy_packed ? c.take(packed_bytes(T, F)) : nullptr;
   float* part = (float*)c.take((size_t)gz_ranges(T) * F * 4);
+  void* room = c.take(linear_bwd_room(T, D, F));
   if (gzb || grad_bias) {
     const int64_t ld = pad8(F);
     RETURN_IF(dtype == MHC_F16
@@ -223,7 +254,7 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
     g.a = {gz, gzs, true};
     g.b = ow;
     g.epi.out = grad_x; g.epi.ld_out = D;
-    RETURN_IF(gemm_run(g, s));
+    RETURN_IF(gemm_run(g, room, s));
   }
   if (grad_weight) {
     RETURN_IF(aligned_operand(&ox, T, D, &c, s));
@@ -231,7 +262,7 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
     g.a = {gz, gzs, false};
     g.b = ox;
     g.epi.out = grad_weight; g.epi.ld_out = D;
-    RETURN_IF(gemm_run(g, s));
+    RETURN_IF(gemm_run(g, room, s));
   }
   return MHC_OK;
 }
@@ -241,6 +272,7 @@ size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
   Carver c{nullptr};
   c.take(packed_bytes(T, F));  // h
+  c.take(ffn_fwd_room(T, D, F));
   if (unaligned) {
     c.take(packed_bytes(T, D));                              // x
     for (int i = 0; i < 2; ++i) c.take(packed_bytes(F, D));  // w_gate, w_up
@@ -270,6 +302,7 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   Carver c{(char*)workspace};
   const int64_t ldh = pad8(F);
   void* h = c.take(packed_bytes(T, F));
+  void* room = c.take(ffn_fwd_room(T, D, F));
   RETURN_IF(aligned_operand(&ox, T, D, &c, s));
   RETURN_IF(aligned_operand(&og, F, D, &c, s));
   RETURN_IF(aligned_operand(&ou, F, D, &c, s));
@@ -283,14 +316,14 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   g.b2 = ou;
   g.epi.act = act; g.epi.out = h; g.epi.ld_out = ldh;
   g.epi.gate = gate; g.epi.up = up; g.epi.ld_gu = gate ? gate_up_stride : 0;
-  RETURN_IF(gemm_run(g, s));
+  RETURN_IF(gemm_run(g, room, s));
   Gemm d;
   d.dtype = dtype;
   d.M = T; d.N = D; d.K = F;
   d.a = {h, ldh, true};
   d.b = od;
   d.epi.out = y; d.epi.ld_out = D;
-  return gemm_run(d, s);
+  return gemm_run(d, room, s);
 }
 
 size_t mhc_gated_ffn_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
@@ -298,6 +331,7 @@ size_t mhc_gated_ffn_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
   Carver c{nullptr};
   for (int i = 0; i < 3; ++i) c.take(packed_bytes(T, F));  // gg, gu, h
+  c.take(ffn_bwd_room(T, D, F));
   if (unaligned) {
     for (int i = 0; i < 2; ++i) c.take(packed_bytes(T, D));  // x, grad_y
     for (int i = 0; i < 2; ++i) c.take(packed_bytes(F, D));  // w_gate, w_up
@@ -338,6 +372,7 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
   void* gg = c.take(packed_bytes(T, F));
   void* gu = c.take(packed_bytes(T, F));
   void* h = c.take(packed_bytes(T, F));
+  void* room = c.take(ffn_bwd_room(T, D, F));
   RETURN_IF(aligned_operand(&oy, T, D, &c, s));
   RETURN_IF(aligned_operand(&od, D, F, &c, s));
   {
@@ -352,7 +387,7 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
     g.epi.ld_gu = gate_up_stride;
     g.epi.gg = gg; g.epi.gu = gu; g.epi.ld_g = ld;
     g.epi.out = h; g.epi.ld_out = ld;
-    RETURN_IF(gemm_run(g, s));
+    RETURN_IF(gemm_run(g, room, s));
   }
   Gemm g;
   g.dtype = dtype;
@@ -366,7 +401,7 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
     g.b3 = ou;
     g.K3 = F;
     g.epi.out = grad_x; g.epi.ld_out = D;
-    RETURN_IF(gemm_run(g, s));
+    RETURN_IF(gemm_run(g, room, s));
     g.K3 = 0;
   }
   if (grad_w_gate || grad_w_up) RETURN_IF(aligned_operand(&ox, T, D, &c, s));
@@ -377,19 +412,19 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
   if (grad_w_gate) {
     g.a = {gg, ld, false};
     g.epi.out = grad_w_gate;
-    RETURN_IF(gemm_run(g, s));
+    RETURN_IF(gemm_run(g, room, s));
   }
   if (grad_w_up) {
     g.a = {gu, ld, false};
     g.epi.out = grad_w_up;
-    RETURN_IF(gemm_run(g, s));
+    RETURN_IF(gemm_run(g, room, s));
   }
   if (grad_w_down) {
     g.M = D; g.N = F;
     g.a = {oy.p, oy.ld, false};
     g.b = {h, ld, false};
     g.epi.out = grad_w_down; g.epi.ld_out = F;
-    RETURN_IF(gemm_run(g, s));
+    RETURN_IF(gemm_run(g, room, s));
   }
   return MHC_OK;
 }
