@@ -2,6 +2,8 @@
 // C[M][N] = A[M][K] B[N][K]^T, with the operator's elementwise work as its epilogue.
 #pragma once
 
+#include <type_traits>
+
 #include "act.cuh"
 
 namespace mhc {
@@ -54,6 +56,10 @@ struct Gemm {
 // sizes alone.
 size_t gemm_ws_bytes(const Gemm& g);
 int gemm_run(const Gemm& g, void* ws, cudaStream_t s);
+
+// For few tokens: K-major operands of any alignment, kEpiLinear or kEpiGated, no third product.
+bool gemv_takes(int64_t M);
+int gemv_run(const Gemm& g, cudaStream_t s);
 
 // Base and rows on 16-byte boundaries, as TMA reads them.
 bool operand_aligned(const Operand& o);

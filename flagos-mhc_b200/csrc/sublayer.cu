@@ -118,13 +118,13 @@ static size_t gemm_room(std::initializer_list<Gemm> gs) {
   return n;
 }
 static size_t linear_fwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 ? 0 : gemm_room({product(kEpiLinear, T, F, D)});
+  return T == 0 || gemv_takes(T) ? 0 : gemm_room({product(kEpiLinear, T, F, D)});
 }
 static size_t linear_bwd_room(int64_t T, int64_t D, int64_t F) {
   return T == 0 ? 0 : gemm_room({product(kEpiLinear, T, D, F), product(kEpiLinear, F, D, T)});
 }
 static size_t ffn_fwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 ? 0 : gemm_room({product(kEpiGated, T, F, D), product(kEpiLinear, T, D, F)});
+  return T == 0 || gemv_takes(T) ? 0 : gemm_room({product(kEpiGated, T, F, D), product(kEpiLinear, T, D, F)});
 }
 static size_t ffn_bwd_room(int64_t T, int64_t D, int64_t F) {
   return T == 0 ? 0 : gemm_room({product(kEpiGatedBwd, T, F, D), product(kEpiLinear, T, D, F, F),
@@ -159,7 +159,7 @@ size_t mhc_linear_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t d
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
   Carver c{nullptr};
   c.take(linear_fwd_room(T, D, F));
-  if (unaligned) {
+  if (unaligned && !gemv_takes(T)) {
     c.take(packed_bytes(T, D));  // x
     c.take(packed_bytes(F, D));  // weight
   }
@@ -187,10 +187,11 @@ int mhc_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   const cudaStream_t s = (cudaStream_t)stream;
   Carver c{(char*)workspace};
   void* room = c.take(linear_fwd_room(T, D, F));
-  RETURN_IF(aligned_operand(&g.a, T, D, &c, s));
-  RETURN_IF(aligned_operand(&g.b, F, D, &c, s));
   g.epi.act = act; g.epi.out = y; g.epi.ld_out = F; g.epi.bias = bias; g.epi.z = z;
   g.epi.res = residual; g.epi.ld_res = residual ? residual_stride : 0;
+  if (gemv_takes(T)) return gemv_run(g, s);
+  RETURN_IF(aligned_operand(&g.a, T, D, &c, s));
+  RETURN_IF(aligned_operand(&g.b, F, D, &c, s));
   return gemm_run(g, room, s);
 }
 
@@ -273,7 +274,7 @@ size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_
   Carver c{nullptr};
   c.take(packed_bytes(T, F));  // h
   c.take(ffn_fwd_room(T, D, F));
-  if (unaligned) {
+  if (unaligned && !gemv_takes(T)) {
     c.take(packed_bytes(T, D));                              // x
     for (int i = 0; i < 2; ++i) c.take(packed_bytes(F, D));  // w_gate, w_up
     c.take(packed_bytes(D, F));                              // w_down
@@ -303,10 +304,13 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   const int64_t ldh = pad8(F);
   void* h = c.take(packed_bytes(T, F));
   void* room = c.take(ffn_fwd_room(T, D, F));
-  RETURN_IF(aligned_operand(&ox, T, D, &c, s));
-  RETURN_IF(aligned_operand(&og, F, D, &c, s));
-  RETURN_IF(aligned_operand(&ou, F, D, &c, s));
-  RETURN_IF(aligned_operand(&od, D, F, &c, s));
+  const bool few = gemv_takes(T);
+  if (!few) {
+    RETURN_IF(aligned_operand(&ox, T, D, &c, s));
+    RETURN_IF(aligned_operand(&og, F, D, &c, s));
+    RETURN_IF(aligned_operand(&ou, F, D, &c, s));
+    RETURN_IF(aligned_operand(&od, D, F, &c, s));
+  }
   Gemm g;
   g.kind = kEpiGated;
   g.dtype = dtype;
@@ -316,14 +320,14 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   g.b2 = ou;
   g.epi.act = act; g.epi.out = h; g.epi.ld_out = ldh;
   g.epi.gate = gate; g.epi.up = up; g.epi.ld_gu = gate ? gate_up_stride : 0;
-  RETURN_IF(gemm_run(g, room, s));
+  RETURN_IF(few ? gemv_run(g, s) : gemm_run(g, room, s));
   Gemm d;
   d.dtype = dtype;
   d.M = T; d.N = D; d.K = F;
   d.a = {h, ldh, true};
   d.b = od;
   d.epi.out = y; d.epi.ld_out = D;
-  return gemm_run(d, room, s);
+  return few ? gemv_run(d, s) : gemm_run(d, room, s);
 }
 
 size_t mhc_gated_ffn_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
