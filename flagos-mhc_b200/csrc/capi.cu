@@ -32,6 +32,7 @@ int post_mix_run(const void* x, const float* h_res, const void* h_out, const flo
                  float* premix, int32_t layers, void* ws, cudaStream_t s);
 int tc_host_device_error();
 int gemm_device_error();
+int gemm_few_device_error();
 int layer_norm_device_error();
 
 static std::atomic<unsigned long long> g_launches{0};
@@ -153,7 +154,8 @@ int mhc_device_status(void) {
   const int g = pre_bwd_tc32_device_error();
   const int h = gemm_device_error();
   const int i = layer_norm_device_error();
-  const int all[9] = {a, b, c, d, e, f, g, h, i};
+  const int j = gemm_few_device_error();
+  const int all[10] = {a, b, c, d, e, f, g, h, i, j};
   for (int v : all)
     if (v != MHC_OK) return v;
   return MHC_OK;

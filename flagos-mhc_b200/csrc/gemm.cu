@@ -40,7 +40,6 @@ struct GemmMaps {
 struct GemmWalk {
   int64_t M, N;                       // of the output
   int32_t tiles_m, tiles_n, nk1, nk;  // K blocks of the first segment, of both
-  int32_t a_k, b_k, a3_k, b3_k;       // operands that are K-major
   int32_t splits;                     // ranges of K, each a unit of work of its own
   float* part;                        // splits > 1: [splits][planes][M][ldp] partial products
   int64_t ldp;
@@ -64,24 +63,6 @@ __device__ __forceinline__ uint32_t leader_addr(const void* p) {
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// a third of a second at least; the longest healthy wait is one tile's products
-constexpr uint32_t kSpin = 1u << 24;
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  for (uint32_t i = 0; i < kSpin; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(tc::smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if ((i & 255) == 255 && *abort) return false;
-  }
-  *abort = 1;
-  return false;
 }
 // load into this CTA's shared memory; the bytes are counted on the leader's barrier
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
@@ -147,7 +128,8 @@ __device__ __forceinline__ Unit unit_at(const GemmWalk& w, int32_t u) {
   return r;
 }
 
-template <typename E, int KIND, int MT>
+// AK, BKM: the operand is K-major
+template <typename E, int KIND, int MT, bool AK, bool BKM>
 __global__ void __launch_bounds__(gk::THREADS, 1)
     gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmWalk w,
                 const __grid_constant__ EpiParams epi) {
@@ -195,98 +177,132 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
 
   const int32_t units = w.tiles_m * w.tiles_n * w.splits;
   const int32_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  // The two issuing loops are warp-wide and unrolled over the ring: barriers, addresses and
+  // descriptors are then constants or uniform registers.
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int32_t i = first; i < units && ok; i += step) {
-        const Unit u = unit_at<MT>(w, i);
-        const int32_t m0 = u.mt * ROWS + (int32_t)rank * BM;
-        const int32_t n0 = dual ? u.nt * BNC : u.nt * 2 * BNC + (int32_t)rank * BNC;
-        for (int32_t kb = u.kb0; kb < u.kb1; ++kb, ++it) {
-          const uint32_t s = it % STAGES;
-          if (!tc2::wait_cluster(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag)) {
-            ok = false;
-            break;
-          }
+    const bool issue = tc::elect_one();
+    const uint32_t base = tc::smem_u32(smem), bar0 = tc2::leader_addr(&full[0]);
+    int32_t i = first, kb = 0, kb1 = 0, m0 = 0, n0 = 0;
+    bool more = true;
+    // the next K block of this cluster's units
+    auto advance = [&]() {
+      if (++kb < kb1) return;
+      if (i >= units) {
+        more = false;
+        return;
+      }
+      const Unit u = unit_at<MT>(w, i);
+      m0 = u.mt * ROWS + (int32_t)rank * BM;
+      n0 = dual ? u.nt * BNC : u.nt * 2 * BNC + (int32_t)rank * BNC;
+      kb = u.kb0;
+      kb1 = u.kb1;
+      i += step;
+    };
+    advance();
+    for (uint32_t ph = 1; more; ph ^= 1) {
+#pragma unroll
+      for (int s = 0; s < STAGES; ++s) {
+        if (!more) break;
+        if (!tc::mbar_wait_warp(&empty[s], ph, abort_flag)) {
+          more = false;
+          break;
+        }
+        const uint32_t bar = bar0 + s * 8;
+        const uint32_t sa = base + s * STAGE_BYTES, sb = sa + MT * A_BYTES;
+        const bool second = kb >= w.nk1;
+        const int32_t k0 = (second ? kb - w.nk1 : kb) * BK;
+        const CUtensorMap* ma = second ? &maps.a3 : &maps.a;
+        const CUtensorMap* mb = second ? &maps.b3 : (dual && rank) ? &maps.b2 : &maps.b;
+        if (issue) {
           if (leader) tc::mbar_arrive_expect_tx(&full[s], 2 * STAGE_BYTES);
-          const uint32_t bar = tc2::leader_addr(&full[s]);
-          const uint32_t sa = tc::smem_u32(smem + s * STAGE_BYTES), sb = sa + MT * A_BYTES;
-          const bool second = kb >= w.nk1;
-          const int32_t k0 = (second ? kb - w.nk1 : kb) * BK;
-          const CUtensorMap* ma = second ? &maps.a3 : &maps.a;
-          const CUtensorMap* mb = second ? &maps.b3 : (dual && rank) ? &maps.b2 : &maps.b;
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             const uint32_t dst = sa + m * A_BYTES;
             const int32_t r0 = m0 + m * 256;
-            if (second ? w.a3_k : w.a_k) {
+            if constexpr (AK) {
               tc2::load_2d(dst, ma, bar, k0, r0);
             } else {
               tc2::load_2d(dst, ma, bar, r0, k0);
               tc2::load_2d(dst + A_BYTES / 2, ma, bar, r0 + 64, k0);
             }
           }
-          if (second ? w.b3_k : w.b_k) {
+          if constexpr (BKM) {
             tc2::load_2d(sb, mb, bar, k0, n0);
           } else {
             tc2::load_2d(sb, mb, bar, n0, k0);
             tc2::load_2d(sb + B_BYTES / 2, mb, bar, n0 + 64, k0);
           }
         }
+        __syncwarp();
+        advance();
       }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs
-    if (lane == 0) {
-      if (leader) {
-        // descriptor step of 16 K elements: 32 bytes of a K-major row, or two 8-row atoms
-        const uint32_t idesc1 = tc::idesc_16<E>(256, 256, !w.a_k, !w.b_k);
-        const uint32_t idesc2 = tc::idesc_16<E>(256, 256, !w.a3_k, !w.b3_k);
-        uint32_t it = 0, j = 0;
-        bool ok = true;
-        for (int32_t i = first; i < units && ok; i += step, ++j) {
-          const Unit u = unit_at<MT>(w, i);
-          // MT = 1: tiles take the two accumulators in turn; MT = 2: each tile takes both
-          const uint32_t buf = MT == 1 ? j & 1 : 0, ph = MT == 1 ? (j >> 1) & 1 : j & 1;
-          if (!tc2::wait_cluster(&tempty[buf], ph ^ 1, abort_flag)) break;
-          if (MT == 2 && !tc2::wait_cluster(&tempty[1], ph ^ 1, abort_flag)) break;
-          tc::tc_fence_after();
-          for (int32_t kb = u.kb0; kb < u.kb1; ++kb, ++it) {
-            const uint32_t s = it % STAGES;
-            if (!tc2::wait_cluster(&full[s], (it / STAGES) & 1, abort_flag)) {
-              ok = false;
+    if (leader) {
+      constexpr uint32_t idesc = tc::idesc_16<E>(256, 256, !AK, !BKM);
+      // descriptor step of 16 K elements: 32 bytes of a K-major row, or two 8-row atoms
+      constexpr uint32_t stepa = AK ? 2 : 128, stepb = BKM ? 2 : 128;
+      const uint32_t base = tc::smem_u32(smem);
+      const uint64_t da0 = tc::smem_desc(base, AK ? 16 : A_BYTES / 2, 1024, tc::kSwizzle128);
+      const uint64_t db0 =
+          tc::smem_desc(base + MT * A_BYTES, BKM ? 16 : B_BYTES / 2, 1024, tc::kSwizzle128);
+      const bool issue = tc::elect_one();
+      int32_t i = first, left = 0;  // K blocks left of this unit
+      uint32_t j = 0, buf = 0, accum = 0;
+      bool more = i < units;
+      for (uint32_t ph = 0; more; ph ^= 1) {
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) {
+          if (left == 0) {  // the next unit
+            if (i >= units) {
+              more = false;
+              break;
+            }
+            const Unit u = unit_at<MT>(w, i);
+            left = u.kb1 - u.kb0;
+            i += step;
+            accum = 0;
+            // MT = 1: units take the two accumulators in turn; MT = 2: each takes both
+            buf = MT == 1 ? j & 1 : 0;
+            const uint32_t tph = (MT == 1 ? (j >> 1) & 1 : j & 1) ^ 1;
+            ++j;
+            if (!tc::mbar_wait_warp(&tempty[buf], tph, abort_flag) ||
+                (MT == 2 && !tc::mbar_wait_warp(&tempty[1], tph, abort_flag))) {
+              more = false;
               break;
             }
             tc::tc_fence_after();
-            const bool second = kb >= w.nk1;
-            const bool ak = second ? w.a3_k : w.a_k, bk = second ? w.b3_k : w.b_k;
-            const uint32_t sa = tc::smem_u32(smem + s * STAGE_BYTES);
-            const uint64_t db = tc::smem_desc(sa + MT * A_BYTES, bk ? 16 : B_BYTES / 2, 1024,
-                                              tc::kSwizzle128);
-            const uint32_t stepa = ak ? 2 : 128, stepb = bk ? 2 : 128;
-            const uint32_t idesc = second ? idesc2 : idesc1;
+          }
+          if (!tc::mbar_wait_warp(&full[s], ph, abort_flag)) {
+            more = false;
+            break;
+          }
+          tc::tc_fence_after();
+          --left;
+          if (issue) {
+            const uint64_t da = da0 + s * (STAGE_BYTES >> 4), db = db0 + s * (STAGE_BYTES >> 4);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-              const uint64_t da = tc::smem_desc(sa + m * A_BYTES, ak ? 16 : A_BYTES / 2, 1024,
-                                                tc::kSwizzle128);
-              const uint32_t d = tmem + (buf + m) * 256;
 #pragma unroll
               for (int k = 0; k < BK / 16; ++k)
-                tc2::mma(d, da + k * stepa, db + k * stepb, idesc, (kb != u.kb0 || k != 0) ? 1u : 0u);
-              if (MT == 2 && kb + 1 == u.kb1) tc2::commit_both(&tfull[m]);
+                tc2::mma(tmem + (buf + m) * 256, da + m * (A_BYTES >> 4) + k * stepa,
+                         db + k * stepb, idesc, k != 0 ? 1u : accum);
+              if (MT == 2 && left == 0) tc2::commit_both(&tfull[m]);
             }
             tc2::commit_both(&empty[s]);
+            if (MT == 1 && left == 0) tc2::commit_both(&tfull[buf]);
           }
-          if (!ok) break;
-          if (MT == 1) tc2::commit_both(&tfull[buf]);
+          accum = 1;
+          __syncwarp();
         }
-        tc2::commit_both(&tdone);  // every MMA has completed before TMEM is freed
       }
-      volatile int never = 0;
-      tc2::wait_cluster(&tdone, 0, &never);
+      if (issue) tc2::commit_both(&tdone);  // every MMA is done before TMEM is freed
     }
+    __syncwarp();
+    volatile int never = 0;
+    tc::mbar_wait(&tdone, 0, &never);
   } else {
     // ---------------------------------------------------------------- epilogue
     // eight warps, four lane quarters: the pair of a quarter splits the columns of the one
@@ -299,7 +315,7 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
     for (int32_t i = first; i < units; i += step, ++j) {
       const Unit u = unit_at<MT>(w, i);
       const uint32_t buf = MT == 1 ? j & 1 : pair, ph = MT == 1 ? (j >> 1) & 1 : j & 1;
-      const bool got = tc2::wait_cluster(&tfull[buf], ph, abort_flag);
+      const bool got = tc::mbar_wait(&tfull[buf], ph, abort_flag);
       if (!__all_sync(0xffffffffu, got)) break;
       tc::tc_fence_after();
       const int64_t row = (int64_t)u.mt * ROWS + (MT == 1 ? 0 : pair * 256) + rank * BM + q * 32 + lane;
@@ -372,7 +388,8 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// How a product is cut: MT accumulators of 256 rows to a tile, `splits` ranges of K.
+// How a product is cut: mt accumulators of 256 rows to a tile, or 0: the form of gemm_few.cu;
+// `splits` ranges of K.
 struct GemmPlan {
   int mt, splits;
 };
@@ -389,8 +406,9 @@ static GemmPlan gemm_plan(const Gemm& g) {
   const int64_t nk = k_blocks(g), clusters = sm_count() / 2;
   const int64_t tn = cdiv(g.N, dual ? gk::BNC : 2 * gk::BNC);
   const double plane = (double)g.M * (double)part_ld(g) * (dual ? 2 : 1);
-  GemmPlan best{1, 1};
-  double best_us = 1e30;
+  GemmPlan best{0, 1};
+  double best_us = few_estimate(g, &best.splits);
+  if (best_us == 0.0) best = {1, 1}, best_us = 1e30;
   for (int mt = 1; mt <= 2; ++mt) {
     if (mt == 2 && g.M <= 256) break;
     const int64_t tiles = cdiv(g.M, 256 * mt) * tn;
@@ -409,7 +427,7 @@ static GemmPlan gemm_plan(const Gemm& g) {
 
 size_t gemm_ws_bytes(const Gemm& g) {
   const GemmPlan p = gemm_plan(g);
-  if (p.splits == 1) return 0;
+  if (p.splits == 1 || p.mt == 0) return 0;
   return align_up((size_t)p.splits * (g.kind == kEpiGated ? 2 : 1) * g.M * part_ld(g) * 4);
 }
 
@@ -431,7 +449,7 @@ static int operand_map(CUtensorMap* m, const Operand& o, int32_t dtype, int64_t 
                                   CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename E, int KIND, int MT>
+template <typename E, int KIND, int MT, bool AK, bool BKM>
 static int gemm_launch(const Gemm& g, int splits, float* part, cudaStream_t s) {
   using namespace gk;
   constexpr bool dual = KIND == kEpiGated;
@@ -451,8 +469,6 @@ static int gemm_launch(const Gemm& g, int splits, float* part, cudaStream_t s) {
   w.tiles_n = (int32_t)cdiv(g.N, dual ? BNC : 2 * BNC);
   w.nk1 = (int32_t)cdiv(g.K, BK);
   w.nk = w.nk1 + (int32_t)cdiv(g.K3, BK);
-  w.a_k = g.a.k_major; w.b_k = g.b.k_major;
-  w.a3_k = g.a3.k_major; w.b3_k = g.b3.k_major;
   w.splits = splits;
   w.part = part;
   w.ldp = part_ld(g);
@@ -461,7 +477,7 @@ static int gemm_launch(const Gemm& g, int splits, float* part, cudaStream_t s) {
   int dev = 0;
   MHC_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    MHC_CUDA_CHECK(cudaFuncSetAttribute((const void*)gemm_kernel<E, KIND, MT>,
+    MHC_CUDA_CHECK(cudaFuncSetAttribute((const void*)gemm_kernel<E, KIND, MT, AK, BKM>,
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
@@ -482,7 +498,7 @@ static int gemm_launch(const Gemm& g, int splits, float* part, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = (!pdl_first_launch() && pdl_enabled()) ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, gemm_kernel<E, KIND, MT>, m, w, g.epi) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, gemm_kernel<E, KIND, MT, AK, BKM>, m, w, g.epi) != cudaSuccess) {
     (void)cudaGetLastError();
     return MHC_ERR_CUDA;
   }
@@ -490,12 +506,13 @@ static int gemm_launch(const Gemm& g, int splits, float* part, cudaStream_t s) {
   return MHC_OK;
 }
 
-template <typename E, int KIND>
+template <typename E, int KIND, bool AK, bool BKM>
 static int gemm_kind(const Gemm& g, void* ws, cudaStream_t s) {
   const GemmPlan p = gemm_plan(g);
+  if (p.mt == 0) return few_run(g, p.splits, s);
   float* part = p.splits > 1 ? (float*)ws : nullptr;
-  const int st = p.mt == 2 ? gemm_launch<E, KIND, 2>(g, p.splits, part, s)
-                           : gemm_launch<E, KIND, 1>(g, p.splits, part, s);
+  const int st = p.mt == 2 ? gemm_launch<E, KIND, 2, AK, BKM>(g, p.splits, part, s)
+                           : gemm_launch<E, KIND, 1, AK, BKM>(g, p.splits, part, s);
   if (st != MHC_OK || !part) return st;
   const int64_t n = g.M * (part_ld(g) / 8);
   launch(gemm_finish_kernel<E, KIND>, (unsigned)std::min<int64_t>(cdiv(n, 256), 8 * sm_count()),
@@ -506,9 +523,12 @@ static int gemm_kind(const Gemm& g, void* ws, cudaStream_t s) {
 
 template <typename E>
 static int gemm_typed(const Gemm& g, void* ws, cudaStream_t s) {
-  if (g.kind == kEpiGated) return gemm_kind<E, kEpiGated>(g, ws, s);
-  if (g.kind == kEpiGatedBwd) return gemm_kind<E, kEpiGatedBwd>(g, ws, s);
-  return gemm_kind<E, kEpiLinear>(g, ws, s);
+  // the operands' orders that the operators meet
+  if (g.kind == kEpiGated) return gemm_kind<E, kEpiGated, true, true>(g, ws, s);
+  if (g.kind == kEpiGatedBwd) return gemm_kind<E, kEpiGatedBwd, true, false>(g, ws, s);
+  if (!g.a.k_major) return gemm_kind<E, kEpiLinear, false, false>(g, ws, s);
+  return g.b.k_major ? gemm_kind<E, kEpiLinear, true, true>(g, ws, s)
+                     : gemm_kind<E, kEpiLinear, true, false>(g, ws, s);
 }
 
 int gemm_run(const Gemm& g0, void* ws, cudaStream_t s) {

@@ -47,15 +47,19 @@ struct Gemm {
   int64_t M = 0, N = 0, K = 0;
   Operand a, b;
   Operand b2;         // kEpiGated: the up projection, N and K as b
-  Operand a3, b3;     // if K3 > 0: adds a3 b3^T (the same M and N) to the product
+  Operand a3, b3;     // if K3 > 0: adds a3 b3^T to the product (M, N and orders as a and b)
   int64_t K3 = 0;
   EpiParams epi;
 };
 
 // Operands must be aligned (operand_aligned).  ws: gemm_ws_bytes, which goes by the kind and the
-// sizes alone.
+// sizes alone (and whether a is K-major).
 size_t gemm_ws_bytes(const Gemm& g);
 int gemm_run(const Gemm& g, void* ws, cudaStream_t s);
+
+// The form with swapped roles (gemm_few.cu): its estimated time and cut, and the run.
+double few_estimate(const Gemm& g, int* splits);
+int few_run(const Gemm& g, int splits, cudaStream_t s);
 
 // For few tokens: K-major operands of any alignment, kEpiLinear or kEpiGated, no third product.
 bool gemv_takes(int64_t M);

@@ -106,8 +106,10 @@ static int aligned_operand(Operand* o, int64_t rows, int64_t cols, Carver* c, cu
   return st;
 }
 // Room for the partial products of the largest of these products (they run one by one).
-static Gemm product(int kind, int64_t M, int64_t N, int64_t K, int64_t K3 = 0) {
+// a_k: whether a (and a3) is K-major, which the plan goes by too.
+static Gemm product(int kind, bool a_k, int64_t M, int64_t N, int64_t K, int64_t K3 = 0) {
   Gemm g;
+  g.a.k_major = g.a3.k_major = a_k;
   g.kind = kind;
   g.M = M; g.N = N; g.K = K; g.K3 = K3;
   return g;
@@ -118,17 +120,17 @@ static size_t gemm_room(std::initializer_list<Gemm> gs) {
   return n;
 }
 static size_t linear_fwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 || gemv_takes(T) ? 0 : gemm_room({product(kEpiLinear, T, F, D)});
+  return T == 0 || gemv_takes(T) ? 0 : gemm_room({product(kEpiLinear, true, T, F, D)});
 }
 static size_t linear_bwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 ? 0 : gemm_room({product(kEpiLinear, T, D, F), product(kEpiLinear, F, D, T)});
+  return T == 0 ? 0 : gemm_room({product(kEpiLinear, true, T, D, F), product(kEpiLinear, false, F, D, T)});
 }
 static size_t ffn_fwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 || gemv_takes(T) ? 0 : gemm_room({product(kEpiGated, T, F, D), product(kEpiLinear, T, D, F)});
+  return T == 0 || gemv_takes(T) ? 0 : gemm_room({product(kEpiGated, true, T, F, D), product(kEpiLinear, true, T, D, F)});
 }
 static size_t ffn_bwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 ? 0 : gemm_room({product(kEpiGatedBwd, T, F, D), product(kEpiLinear, T, D, F, F),
-                                 product(kEpiLinear, F, D, T), product(kEpiLinear, D, F, T)});
+  return T == 0 ? 0 : gemm_room({product(kEpiGatedBwd, true, T, F, D), product(kEpiLinear, true, T, D, F, F),
+                                 product(kEpiLinear, false, F, D, T), product(kEpiLinear, false, D, F, T)});
 }
 
 static bool any_unaligned(std::initializer_list<Operand> ops) {
