@@ -5,6 +5,7 @@ library is missing or the tensors are not on an sm_100 GPU, the call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -166,8 +167,22 @@ def dtype_code(dt):
         raise TypeError(f"FlagOS_mhc: unsupported dtype {dt}; expected float32/float16/bfloat16")
 
 
+# torch's own raw-handle getter (0.1 us; building a Stream object takes 2 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_no_guard = contextlib.nullcontext()
+
+
 def stream_of(t):
+    if _raw_stream is not None:
+        return ctypes.c_void_p(_raw_stream(t.device.index))
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def device_guard(device):
+    """torch.cuda.device(device), or nothing where it is the current device already."""
+    if torch.cuda.current_device() == device.index:
+        return _no_guard
+    return torch.cuda.device(device)
 
 
 def check(status: int, what: str):
@@ -211,6 +226,8 @@ def act_code(name):
 def rows(t, width):
     """(tensor, row stride in elements) of t = (T, width) or (B, S, width), read in place if its
     rows share one stride, packed first otherwise."""
+    if t.is_contiguous():
+        return t, width
     ts = token_view(t, 1, width)
     if ts is None:
         return t.contiguous(), width

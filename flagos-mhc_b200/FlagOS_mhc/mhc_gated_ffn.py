@@ -52,7 +52,7 @@ def mhc_gated_ffn(x, w_gate, w_up, w_down, activation="silu", need_backward=Fals
     if need_backward:
         gate, up = torch.empty(2, T, ld, dtype=x.dtype, device=dev)[:, :, :F].unbind(0)
     L = _C.lib()
-    with torch.cuda.device(dev):
+    with _C.device_guard(dev):
         nbytes = L.mhc_gated_ffn_fwd_workspace_bytes(
             T, D, F, code, _C.unaligned((xf, xs), (gf, gs), (uf, us), (df, ds)))
         ws, wp = _C.workspace(nbytes, dev)

@@ -38,7 +38,7 @@ def mhc_gated_ffn_backward(x, w_gate, w_up, w_down, gate, up, grad_y, activation
     shapes = (x.shape, (F, D), (F, D), (D, F))
     outs = [torch.empty(s, **kw) if n else None for s, n in zip(shapes, need_grads)]
     L = _C.lib()
-    with torch.cuda.device(x.device):
+    with _C.device_guard(x.device):
         nbytes = L.mhc_gated_ffn_bwd_workspace_bytes(
             T, D, F, code, _C.unaligned((xf, xs), (wg, wgs), (wu, wus), (wd, wds), (gf, gs)))
         ws, wp = _C.workspace(nbytes, x.device)

@@ -55,7 +55,7 @@ def mhc_layer_norm(x, weight=None, bias=None, eps=1e-5, need_backward=False):
     if need_backward:
         mean = torch.empty(T, dtype=torch.float32, device=dev)
         rstd = torch.empty(T, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _C.device_guard(dev):
         st = _C.lib().mhc_layer_norm_fwd(_C.ptr(xf), xs, _C.ptr(w), _C.ptr(b), T, D, code,
                                          float(eps), _C.ptr(y), _C.ptr(mean), _C.ptr(rstd),
                                          _C.stream_of(x))

@@ -35,7 +35,7 @@ def mhc_layer_norm_backward(x, weight, mean, rstd, grad_y, need_param_grads=True
     gw = gb = ws = wp = None
     nbytes = 0
     L = _C.lib()
-    with torch.cuda.device(dev):
+    with _C.device_guard(dev):
         if need_param_grads:
             gw, gb = torch.empty(2, D, dtype=torch.float32, device=dev).unbind(0)
             nbytes = L.mhc_layer_norm_bwd_workspace_bytes(T, D, code)

@@ -58,7 +58,7 @@ def mhc_linear(x, weight, bias=None, residual=None, activation="none", need_back
     y = torch.empty(out_shape, dtype=x.dtype, device=dev)
     z = torch.empty(out_shape, dtype=x.dtype, device=dev) if need_backward and act else None
     L = _C.lib()
-    with torch.cuda.device(dev):
+    with _C.device_guard(dev):
         nbytes = L.mhc_linear_fwd_workspace_bytes(T, D, F, code,
                                                   _C.unaligned((xf, xs), (wf, wstr)))
         ws, wp = _C.workspace(nbytes, dev)

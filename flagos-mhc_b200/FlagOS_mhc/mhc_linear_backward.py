@@ -38,7 +38,7 @@ def mhc_linear_backward(x, weight, z, grad_y, activation="none", need_x_grad=Tru
     gw = torch.empty(F, D, **kw) if need_weight_grad else None
     gb = torch.empty(F, **kw) if need_bias_grad else None
     L = _C.lib()
-    with torch.cuda.device(x.device):
+    with _C.device_guard(x.device):
         nbytes = L.mhc_linear_bwd_workspace_bytes(
             T, D, F, code, act, _C.unaligned((xf, xs), (wf, wstr), (gf, gs)))
         ws, wp = _C.workspace(nbytes, x.device)

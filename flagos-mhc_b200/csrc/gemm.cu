@@ -388,38 +388,39 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// How a product is cut: mt accumulators of 256 rows to a tile, or 0: the form of gemm_few.cu;
-// `splits` ranges of K.
+// How a product is cut: mt accumulators of 256 rows to a tile, or 0: the form of gemm_few.cu
+// with nt tokens to a tile; `splits` ranges of K.
 struct GemmPlan {
-  int mt, splits;
+  int mt, splits, nt;
 };
 static int64_t k_blocks(const Gemm& g) { return cdiv(g.K, gk::BK) + cdiv(g.K3, gk::BK); }
 static int64_t part_ld(const Gemm& g) { return cdiv(g.N, 32) * 32; }
 
-// The cut whose estimated time is least.  Measured on full grids: 0.50 us to a K block of a
-// 256-row tile, 0.86 us of a 512-row one (which reads B half as often for its work, and whose
+// The cut whose estimated time (us) is least.  Measured: 7 us to start and end a launch; 0.36 us
+// to a K block of a 256-row tile and 0.73 us of a 512-row one in a short run, 0.50 and 0.86 us
+// under the power cap (the 512-row tile reads B half as often for its work).  The 512-row tile's
 // epilogue, with no accumulators left for the next tile, stands alone: 2 us, 3 us with a gate,
-// 20 us with the gate's backward).  A cut in K writes and reads fp32 partials (at 4 TB/s) and
+// 20 us with the gate's backward.  A cut in K writes and reads fp32 partials (at 4 TB/s) and
 // takes another launch (3 us).
 static GemmPlan gemm_plan(const Gemm& g) {
   const bool dual = g.kind == kEpiGated;
   const int64_t nk = k_blocks(g), clusters = sm_count() / 2;
   const int64_t tn = cdiv(g.N, dual ? gk::BNC : 2 * gk::BNC);
   const double plane = (double)g.M * (double)part_ld(g) * (dual ? 2 : 1);
-  GemmPlan best{0, 1};
-  double best_us = few_estimate(g, &best.splits);
-  if (best_us == 0.0) best = {1, 1}, best_us = 1e30;
+  GemmPlan best{0, 1, 0};
+  double best_us = few_estimate(g, &best.nt, &best.splits);
+  if (best_us == 0.0) best = {1, 1, 0}, best_us = 1e30;
   for (int mt = 1; mt <= 2; ++mt) {
     if (mt == 2 && g.M <= 256) break;
     const int64_t tiles = cdiv(g.M, 256 * mt) * tn;
-    const double per_k = mt == 1 ? 0.50 : 0.86;
+    const double per_k = mt == 1 ? 0.40 : 0.75;
     const double tail = mt == 1 ? 1.0 : g.kind == kEpiLinear ? 2.0 : dual ? 3.0 : 20.0;
     for (int sp = 1; sp <= 16; ++sp) {
       if (sp > 1 && (nk < 4 * sp || plane * sp * 4 > 1e9)) break;
       const double waves = (double)cdiv(tiles * sp, clusters);
-      double us = waves * ((double)cdiv(nk, sp) * per_k + tail);
+      double us = 7.0 + waves * ((double)cdiv(nk, sp) * per_k + tail);
       if (sp > 1) us += 3.0 + plane * sp * 8 / 4e6;
-      if (us < best_us) best_us = us, best = {mt, sp};
+      if (us < best_us) best_us = us, best = {mt, sp, 0};
     }
   }
   return best;
@@ -509,7 +510,7 @@ static int gemm_launch(const Gemm& g, int splits, float* part, cudaStream_t s) {
 template <typename E, int KIND, bool AK, bool BKM>
 static int gemm_kind(const Gemm& g, void* ws, cudaStream_t s) {
   const GemmPlan p = gemm_plan(g);
-  if (p.mt == 0) return few_run(g, p.splits, s);
+  if (p.mt == 0) return few_run(g, p.nt, p.splits, s);
   float* part = p.splits > 1 ? (float*)ws : nullptr;
   const int st = p.mt == 2 ? gemm_launch<E, KIND, 2, AK, BKM>(g, p.splits, part, s)
                            : gemm_launch<E, KIND, 1, AK, BKM>(g, p.splits, part, s);

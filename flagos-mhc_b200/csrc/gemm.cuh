@@ -57,12 +57,12 @@ struct Gemm {
 size_t gemm_ws_bytes(const Gemm& g);
 int gemm_run(const Gemm& g, void* ws, cudaStream_t s);
 
-// The form with swapped roles (gemm_few.cu): its estimated time and cut, and the run.
-double few_estimate(const Gemm& g, int* splits);
-int few_run(const Gemm& g, int splits, cudaStream_t s);
+// The form with swapped roles (gemm_few.cu): its estimated time, tile and cut, and the run.
+double few_estimate(const Gemm& g, int* nt, int* splits);
+int few_run(const Gemm& g, int nt, int splits, cudaStream_t s);
 
 // For few tokens: K-major operands of any alignment, kEpiLinear or kEpiGated, no third product.
-bool gemv_takes(int64_t M);
+bool gemv_takes(int64_t M, int64_t N, int64_t K);
 int gemv_run(const Gemm& g, cudaStream_t s);
 
 // Base and rows on 16-byte boundaries, as TMA reads them.

@@ -297,33 +297,38 @@ static int few_launch(const Gemm& g, int splits, cudaStream_t s) {
   return MHC_OK;
 }
 
-// tokens to a tile
-static int few_nt(const Gemm& g) {
-  return g.M <= 32 ? 32 : g.M <= 64 ? 64 : (g.M <= 128 || g.kind == kEpiGated) ? 128 : 256;
-}
-
-// Estimated time (us) of the best cut in K, 0 if this form does not take the product.
-double few_estimate(const Gemm& g, int* splits) {
+// The tile and the cut in K whose estimated time (us) is least; 0 if this form does not take the
+// product.  Measured: 4 us to start and end a launch; to a K block 0.17 us, or its bytes at 130
+// GB/s an SM and 14 TB/s in all; at a tile's end 0.6 us and 0.016 us a token; the weights at 6.4 TB/s after 6 us.
+// (Clusters of 8 CTAs of this size leave SMs empty: 1024 -> 2048 features, T=128: 22 us against
+// 9.6 with 2.)
+double few_estimate(const Gemm& g, int* nt_best, int* splits) {
   if (!g.a.k_major) return 0.0;
-  const int nt = few_nt(g), W = g.kind == kEpiGated ? 2 : 1;
+  const int W = g.kind == kEpiGated ? 2 : 1;
   const int64_t nk = cdiv(g.K, fk::BK) + cdiv(g.K3, fk::BK);
-  const int64_t tiles = cdiv(g.N, fk::BM) * cdiv(g.M, nt);
-  // a K block: its bytes at an SM's share of HBM (or a little more, with idle SMs), or its MMAs
-  const double bytes = W * 16384.0 + nt * 128.0;
-  const double per_k = std::max(bytes / 60e3, W * nt * 0.0016);
+  const double hbm = 6.0 + (double)W * g.N * (g.K + g.K3) * 2 / 6.4e6;
   double best = 1e30;
-  for (int sp = 1; sp <= 8; sp *= 2) {
-    if (sp > 1 && nk < 2 * sp) break;
-    const double waves = (double)cdiv(tiles * sp, sm_count());
-    const double us = 2.0 + waves * (cdiv(nk, sp) * per_k + 1.0 + W * nt * 0.01) + (sp > 1 ? 1.0 : 0.0);
-    if (us < best) best = us, *splits = sp;
+  for (int nt = 32; nt <= (W == 2 ? 128 : 256); nt *= 2) {
+    if (nt > 32 && nt >= 2 * g.M) break;
+    const int64_t tiles = cdiv(g.N, fk::BM) * cdiv(g.M, nt);
+    const double bytes = W * 16384.0 + nt * 128.0;
+    for (int sp = 1; sp <= 4; sp *= 2) {
+      if (sp > 1 && nk < 2 * sp) break;
+      const double waves = (double)cdiv(tiles * sp, sm_count());
+      const double active = (double)std::min<int64_t>(tiles * sp, sm_count());
+      const double per_k = std::max(0.17 * W, std::max(bytes / 130e3, bytes * active / 14e6));
+      double us = 4.0 + (sp > 1 ? 0.8 : 0.0) +
+                  waves * ((double)cdiv(nk, sp) * per_k + 0.6 + 0.016 * W * nt);
+      us = std::max(us, hbm);
+      if (us < best) best = us, *nt_best = nt, *splits = sp;
+    }
   }
   return best;
 }
 
 template <typename E, int KIND, bool AK>
-static int few_kind(const Gemm& g, int splits, cudaStream_t s) {
-  switch (few_nt(g)) {
+static int few_kind(const Gemm& g, int nt, int splits, cudaStream_t s) {
+  switch (nt) {
     case 32: return few_launch<E, KIND, 32, AK>(g, splits, s);
     case 64: return few_launch<E, KIND, 64, AK>(g, splits, s);
     case 128: return few_launch<E, KIND, 128, AK>(g, splits, s);
@@ -333,15 +338,15 @@ static int few_kind(const Gemm& g, int splits, cudaStream_t s) {
   }
 }
 template <typename E>
-static int few_typed(const Gemm& g, int splits, cudaStream_t s) {
-  if (g.kind == kEpiGated) return few_kind<E, kEpiGated, true>(g, splits, s);
-  if (g.kind == kEpiGatedBwd) return few_kind<E, kEpiGatedBwd, false>(g, splits, s);
-  return g.b.k_major ? few_kind<E, kEpiLinear, true>(g, splits, s)
-                     : few_kind<E, kEpiLinear, false>(g, splits, s);
+static int few_typed(const Gemm& g, int nt, int splits, cudaStream_t s) {
+  if (g.kind == kEpiGated) return few_kind<E, kEpiGated, true>(g, nt, splits, s);
+  if (g.kind == kEpiGatedBwd) return few_kind<E, kEpiGatedBwd, false>(g, nt, splits, s);
+  return g.b.k_major ? few_kind<E, kEpiLinear, true>(g, nt, splits, s)
+                     : few_kind<E, kEpiLinear, false>(g, nt, splits, s);
 }
-int few_run(const Gemm& g, int splits, cudaStream_t s) {
-  return g.dtype == MHC_F16 ? few_typed<__half>(g, splits, s)
-                            : few_typed<__nv_bfloat16>(g, splits, s);
+int few_run(const Gemm& g, int nt, int splits, cudaStream_t s) {
+  return g.dtype == MHC_F16 ? few_typed<__half>(g, nt, splits, s)
+                            : few_typed<__nv_bfloat16>(g, nt, splits, s);
 }
 
 int gemm_few_device_error() { return read_and_clear_tu_error(); }

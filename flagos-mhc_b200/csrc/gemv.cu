@@ -172,7 +172,12 @@ static int gemv_typed(const Gemm& g, cudaStream_t s) {
   return g.kind == kEpiGated ? gemv_kind<E, kEpiGated>(g, s) : gemv_kind<E, kEpiLinear>(g, s);
 }
 
-bool gemv_takes(int64_t M) { return M <= 16; }
+// 9 to 16 tokens read a second set of B fragments: the tcgen05 form is faster there from 64 MB of
+// weights on (4096 -> 16384 features, T=16: 29.0 us here, 26.4 us there; 4096 -> 4096: 9.5 us here,
+// 11.1 us there).
+bool gemv_takes(int64_t M, int64_t N, int64_t K) {
+  return M <= 8 || (M <= 16 && N * K < (int64_t)1 << 25);
+}
 
 int gemv_run(const Gemm& g0, cudaStream_t s) {
   Gemm g = g0;

@@ -120,13 +120,13 @@ static size_t gemm_room(std::initializer_list<Gemm> gs) {
   return n;
 }
 static size_t linear_fwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 || gemv_takes(T) ? 0 : gemm_room({product(kEpiLinear, true, T, F, D)});
+  return T == 0 || gemv_takes(T, F, D) ? 0 : gemm_room({product(kEpiLinear, true, T, F, D)});
 }
 static size_t linear_bwd_room(int64_t T, int64_t D, int64_t F) {
   return T == 0 ? 0 : gemm_room({product(kEpiLinear, true, T, D, F), product(kEpiLinear, false, F, D, T)});
 }
 static size_t ffn_fwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 || gemv_takes(T) ? 0 : gemm_room({product(kEpiGated, true, T, F, D), product(kEpiLinear, true, T, D, F)});
+  return T == 0 || gemv_takes(T, F, D) ? 0 : gemm_room({product(kEpiGated, true, T, F, D), product(kEpiLinear, true, T, D, F)});
 }
 static size_t ffn_bwd_room(int64_t T, int64_t D, int64_t F) {
   return T == 0 ? 0 : gemm_room({product(kEpiGatedBwd, true, T, F, D), product(kEpiLinear, true, T, D, F, F),
@@ -161,7 +161,7 @@ size_t mhc_linear_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t d
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
   Carver c{nullptr};
   c.take(linear_fwd_room(T, D, F));
-  if (unaligned && !gemv_takes(T)) {
+  if (unaligned && !gemv_takes(T, F, D)) {
     c.take(packed_bytes(T, D));  // x
     c.take(packed_bytes(F, D));  // weight
   }
@@ -191,7 +191,7 @@ int mhc_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   void* room = c.take(linear_fwd_room(T, D, F));
   g.epi.act = act; g.epi.out = y; g.epi.ld_out = F; g.epi.bias = bias; g.epi.z = z;
   g.epi.res = residual; g.epi.ld_res = residual ? residual_stride : 0;
-  if (gemv_takes(T)) return gemv_run(g, s);
+  if (gemv_takes(T, F, D)) return gemv_run(g, s);
   RETURN_IF(aligned_operand(&g.a, T, D, &c, s));
   RETURN_IF(aligned_operand(&g.b, F, D, &c, s));
   return gemm_run(g, room, s);
@@ -276,7 +276,7 @@ size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_
   Carver c{nullptr};
   c.take(packed_bytes(T, F));  // h
   c.take(ffn_fwd_room(T, D, F));
-  if (unaligned && !gemv_takes(T)) {
+  if (unaligned && !gemv_takes(T, F, D)) {
     c.take(packed_bytes(T, D));                              // x
     for (int i = 0; i < 2; ++i) c.take(packed_bytes(F, D));  // w_gate, w_up
     c.take(packed_bytes(D, F));                              // w_down
@@ -306,7 +306,7 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   const int64_t ldh = pad8(F);
   void* h = c.take(packed_bytes(T, F));
   void* room = c.take(ffn_fwd_room(T, D, F));
-  const bool few = gemv_takes(T);
+  const bool few = gemv_takes(T, F, D);
   if (!few) {
     RETURN_IF(aligned_operand(&ox, T, D, &c, s));
     RETURN_IF(aligned_operand(&og, F, D, &c, s));
