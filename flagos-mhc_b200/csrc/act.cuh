@@ -15,10 +15,32 @@ __device__ __forceinline__ float sigmoid_fast(float z) {
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluK = 0.044715f;
 
+// The normal distribution function, and e = exp(-z^2 / 2).  With x = |z| / sqrt(2),
+// erfc(x) = e t P(t), t = 1 / (1 + 0.38 x): P is a fit of erfcx(x) / t of degree 6, weighted for
+// the relative error over x = 0 .. 9.5 (1.1e-6; 1.4e-6 with fp32 arithmetic), so the negative tail
+// keeps its accuracy.  The backward needs e anyway; with erfcf it was bound by its instructions
+// (65536 x 4096 elements: 606 us, 312 us for silu).
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  e = __expf(-0.5f * z * z);
+  const float t = __fdividef(1.f, fmaf(0.38f * 0.7071067811865476f, fabsf(z), 1.f));
+  float p = -0.1250499039888382f;
+  p = fmaf(p, t, 0.3346192240715027f);
+  p = fmaf(p, t, -0.06771065294742584f);
+  p = fmaf(p, t, 0.2460743486881256f);
+  p = fmaf(p, t, 0.18135355412960052f);
+  p = fmaf(p, t, 0.2164105623960495f);
+  p = fmaf(p, t, 0.21430183947086334f);
+  const float q = 0.5f * t * p * e;
+  return z < 0.f ? q : 1.f - q;
+}
+
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (ACT == MHC_ACT_RELU) return z < 0.f ? 0.f : z;  // NaN passes
-  if constexpr (ACT == MHC_ACT_GELU) return 0.5f * z * erfcf(-0.7071067811865476f * z);
+  if constexpr (ACT == MHC_ACT_GELU) {
+    float e;
+    return z * normal_cdf(z, e);
+  }
   // 0.5 z (1 + tanh(u)) = z sigmoid(2u)
   if constexpr (ACT == MHC_ACT_GELU_TANH)
     return z * sigmoid_fast(2.f * kGeluC * z * fmaf(kGeluK * z, z, 1.f));
@@ -33,9 +55,10 @@ __device__ __forceinline__ void act_both(float z, float& a, float& da) {
     a = z < 0.f ? 0.f : z;
     da = z > 0.f ? 1.f : (z == z ? 0.f : z);
   } else if constexpr (ACT == MHC_ACT_GELU) {
-    const float cdf = 0.5f * erfcf(-0.7071067811865476f * z);
+    float e;
+    const float cdf = normal_cdf(z, e);
     a = z * cdf;
-    da = fmaf(z * 0.3989422804014327f, __expf(-0.5f * z * z), cdf);
+    da = fmaf(z * 0.3989422804014327f, e, cdf);
   } else if constexpr (ACT == MHC_ACT_GELU_TANH) {
     const float s = sigmoid_fast(2.f * kGeluC * z * fmaf(kGeluK * z, z, 1.f));
     a = z * s;

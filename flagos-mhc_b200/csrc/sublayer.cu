@@ -8,52 +8,111 @@
 namespace mhc {
 
 // ------------------------------------------------------------------ gz and grad_bias
-// gz = grad_y * act'(z) in dtype and, per row range, the column sums of the unrounded gz.
-static constexpr int kGzRanges = 64;
-static int gz_ranges(int64_t T) { return (int)(T < kGzRanges * 64 ? cdiv(T, 64) : kGzRanges); }
+// gz = grad_y * act'(z) in dtype and, per row range, the column sums of the unrounded gz: bound
+// by HBM.  A block takes 256 columns of a row range, 8 to a thread (a 16-byte pack where the rows
+// allow it), its warps every eighth row; their sums are added in order.
+// About 4096 blocks, of at least 32 rows (65536 x 4096, silu: 271 us with 256 ranges, 306 us with
+// 64; two or four rows of a warp at once took 380 and 473 us).
+static int gz_ranges(int64_t T, int64_t F) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(256, 4096 / cdiv(F, 256)));
+  return (int)std::min<int64_t>(cdiv(T, 32), most);
+}
 
-template <typename E, int ACT>
+template <typename E, int ACT, bool VEC>
 __global__ void __launch_bounds__(256)
     act_bwd_kernel(const E* __restrict__ z, int64_t zs, const E* __restrict__ gy, int64_t gs,
                    int64_t T, int64_t F, E* __restrict__ gz, int64_t ld, float* __restrict__ part) {
   pdl_enter();
-  const int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (f >= F) return;
+  __shared__ float red[8][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c0 = (int64_t)blockIdx.x * 256;
   const int64_t t0 = T * blockIdx.y / gridDim.y, t1 = T * (blockIdx.y + 1) / gridDim.y;
-  float s = 0.f;
-  for (int64_t t = t0; t < t1; ++t) {
-    float v = ld1<E>(gy + t * gs + f);
-    if constexpr (ACT != MHC_ACT_NONE) {
-      float a, da;
-      act_both<ACT>(ld1<E>(z + t * zs + f), a, da);
-      v *= da;
+  // element e of this thread is column c0 + 8 lane + e, or c0 + lane + 32 e
+  const int64_t c = c0 + (VEC ? 8 * lane : lane);
+  constexpr int STEP = VEC ? 1 : 32;
+  float s[8] = {};
+  const int64_t tn = VEC && c >= F ? t0 : t1;  // F is a multiple of 8 with VEC
+  for (int64_t t = t0 + warp; t < tn; t += 8) {
+    float v[8], zv[8];
+    if constexpr (VEC) {
+      widen<E>(ld_stream(gy + t * gs + c), v);
+      if constexpr (ACT != MHC_ACT_NONE) widen<E>(ld_stream(z + t * zs + c), zv);
+    } else {
+      E a[8], b[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t k = min(c + 32 * e, F - 1);
+        a[e] = gy[t * gs + k];
+        if constexpr (ACT != MHC_ACT_NONE) b[e] = z[t * zs + k];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = c + 32 * e < F ? from_e(a[e]) : 0.f;
+        if constexpr (ACT != MHC_ACT_NONE) zv[e] = from_e(b[e]);
+      }
     }
-    if (gz) st1<E>(gz + t * ld + f, v);
-    s += v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (ACT != MHC_ACT_NONE) {
+        float av, da;
+        act_both<ACT>(zv[e], av, da);
+        v[e] *= da;
+      }
+      if (VEC || c + 32 * e < F) s[e] += v[e];
+    }
+    if (gz) {
+      if constexpr (VEC) {
+        *reinterpret_cast<uint4*>(gz + t * ld + c) = narrow<E>(v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + 32 * e < F) gz[t * ld + c + 32 * e] = to_e<E>(v[e]);
+      }
+    }
   }
-  if (part) part[(int64_t)blockIdx.y * F + f] = s;
+  if (!part) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) red[warp][(VEC ? 8 * lane : lane) + STEP * e] = s[e];
+  __syncthreads();
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum += red[k][threadIdx.x];
+  if (c0 + threadIdx.x < F) part[(int64_t)blockIdx.y * F + c0 + threadIdx.x] = sum;
 }
 
+// 32 columns per block; eight contiguous ranges of partials side by side, then in order
 template <typename E>
 __global__ void __launch_bounds__(256)
     bias_finish_kernel(const float* __restrict__ part, int ranges, int64_t F, E* __restrict__ gb) {
   pdl_enter();
-  const int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (f >= F) return;
+  __shared__ float sum[8][33];
+  const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5;
+  const int64_t f = (int64_t)blockIdx.x * 32 + lane;
   Kahan k;
-  for (int i = 0; i < ranges; ++i) k.add(part[(int64_t)i * F + f]);
-  st1<E>(gb + f, k.s);
+  if (f < F) {
+#pragma unroll 8
+    for (int i = ranges * seg / 8; i < ranges * (seg + 1) / 8; ++i) k.add(part[(int64_t)i * F + f]);
+  }
+  sum[seg][lane] = k.s;
+  __syncthreads();
+  if (seg == 0 && f < F) {
+    Kahan t;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t.add(sum[i][lane]);
+    st1<E>(gb + f, t.s);
+  }
 }
 
 template <typename E>
 static int act_bwd_run(int act, const void* z, int64_t zs, const void* gy, int64_t gs, int64_t T,
                        int64_t F, void* gz, int64_t ld, void* gb, float* part, cudaStream_t s) {
-  const int ranges = gz_ranges(T);
+  const int ranges = gz_ranges(T, F);
   const dim3 grid((unsigned)cdiv(F, 256), ranges);
   float* pt = gb ? part : nullptr;
-#define MHC_GZ(A)                                                                              \
-  (launch(act_bwd_kernel<E, A>, grid, 256, 0, s, (const E*)z, zs, (const E*)gy, gs, T, F, (E*)gz, \
-          ld, pt),                                                                              \
+  const bool vec = aligned16(z) && zs % 8 == 0 && aligned16(gy) && gs % 8 == 0 && F % 8 == 0;
+#define MHC_GZ(A)                                                                               \
+  (launch(vec ? act_bwd_kernel<E, A, true> : act_bwd_kernel<E, A, false>, grid, 256, 0, s,      \
+          (const E*)z, zs, (const E*)gy, gs, T, F, (E*)gz, ld, pt),                             \
    MHC_OK)
   auto run = [&]() -> int { MHC_DISPATCH_ACT(act, MHC_GZ) };
 #undef MHC_GZ
@@ -61,7 +120,7 @@ static int act_bwd_run(int act, const void* z, int64_t zs, const void* gy, int64
   if (st != MHC_OK) return st;
   MHC_LAUNCH_CHECK();
   if (gb) {
-    launch(bias_finish_kernel<E>, (unsigned)cdiv(F, 256), 256, 0, s, (const float*)part, ranges, F,
+    launch(bias_finish_kernel<E>, (unsigned)cdiv(F, 32), 256, 0, s, (const float*)part, ranges, F,
            (E*)gb);
     MHC_LAUNCH_CHECK();
   }
@@ -202,7 +261,7 @@ size_t mhc_linear_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t d
   if (sub_check(T, D, F, dtype, act) != MHC_OK) return 0;
   Carver c{nullptr};
   if (act != MHC_ACT_NONE || unaligned) c.take(packed_bytes(T, F));  // gz
-  c.take((size_t)gz_ranges(T) * F * 4);
+  c.take((size_t)gz_ranges(T, F) * F * 4);
   c.take(linear_bwd_room(T, D, F));
   if (unaligned) {
     c.take(packed_bytes(T, D));  // x
@@ -237,7 +296,7 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   Carver c{(char*)workspace};
   // without an activation gz is grad_y, copied only where its rows are unaligned
   void* gzb = act != MHC_ACT_NONE || gy_packed ? c.take(packed_bytes(T, F)) : nullptr;
-  float* part = (float*)c.take((size_t)gz_ranges(T) * F * 4);
+  float* part = (float*)c.take((size_t)gz_ranges(T, F) * F * 4);
   void* room = c.take(linear_bwd_room(T, D, F));
   if (gzb || grad_bias) {
     const int64_t ld = pad8(F);
