@@ -238,7 +238,7 @@ def unaligned(*pairs):
     """1 if any (matrix, row stride) does not start its rows on 16-byte boundaries, else 0
     (2-byte elements)."""
     for t, ld in pairs:
-        if (t.data_ptr() | (ld << 1)) & 15:
+        if t is not None and (t.data_ptr() | (ld << 1)) & 15:
             return 1
     return 0
 

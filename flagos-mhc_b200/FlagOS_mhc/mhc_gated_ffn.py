@@ -54,7 +54,7 @@ def mhc_gated_ffn(x, w_gate, w_up, w_down, activation="silu", need_backward=Fals
     L = _C.lib()
     with _C.device_guard(dev):
         nbytes = L.mhc_gated_ffn_fwd_workspace_bytes(
-            T, D, F, code, _C.unaligned((xf, xs), (gf, gs), (uf, us), (df, ds)))
+            T, D, F, code, _C.unaligned((xf, xs), (gf, gs), (uf, us), (df, ds), (y, D)))
         ws, wp = _C.workspace(nbytes, dev)
         st = L.mhc_gated_ffn_fwd(_C.ptr(xf), xs, _C.ptr(gf), gs, _C.ptr(uf), us, _C.ptr(df), ds, T,
                                  D, F, code, act, _C.ptr(y), _C.ptr(gate), _C.ptr(up), ld, wp,

@@ -40,7 +40,7 @@ def mhc_gated_ffn_backward(x, w_gate, w_up, w_down, gate, up, grad_y, activation
     L = _C.lib()
     with _C.device_guard(x.device):
         nbytes = L.mhc_gated_ffn_bwd_workspace_bytes(
-            T, D, F, code, _C.unaligned((xf, xs), (wg, wgs), (wu, wus), (wd, wds), (gf, gs)))
+            T, D, F, code, _C.unaligned((xf, xs), (wg, wgs), (wu, wus), (wd, wds), (gf, gs), (wg, D), (wd, F)))
         ws, wp = _C.workspace(nbytes, x.device)
         st = L.mhc_gated_ffn_bwd(_C.ptr(xf), xs, _C.ptr(wg), wgs, _C.ptr(wu), wus, _C.ptr(wd), wds,
                                  _C.ptr(ga), _C.ptr(ua), gas, _C.ptr(gf), gs, T, D, F, code, act,

@@ -60,7 +60,7 @@ def mhc_linear(x, weight, bias=None, residual=None, activation="none", need_back
     L = _C.lib()
     with _C.device_guard(dev):
         nbytes = L.mhc_linear_fwd_workspace_bytes(T, D, F, code,
-                                                  _C.unaligned((xf, xs), (wf, wstr)))
+                                                  _C.unaligned((xf, xs), (wf, wstr), (rf, rs), (y, F)))
         ws, wp = _C.workspace(nbytes, dev)
         st = L.mhc_linear_fwd(_C.ptr(xf), xs, _C.ptr(wf), wstr, _C.ptr(bf), _C.ptr(rf), rs, T, D,
                               F, code, act, _C.ptr(y), _C.ptr(z), wp, nbytes, _C.stream_of(x))

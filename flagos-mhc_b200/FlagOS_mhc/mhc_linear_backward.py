@@ -40,7 +40,7 @@ def mhc_linear_backward(x, weight, z, grad_y, activation="none", need_x_grad=Tru
     L = _C.lib()
     with _C.device_guard(x.device):
         nbytes = L.mhc_linear_bwd_workspace_bytes(
-            T, D, F, code, act, _C.unaligned((xf, xs), (wf, wstr), (gf, gs)))
+            T, D, F, code, act, _C.unaligned((xf, xs), (wf, wstr), (gf, gs), (gx, D), (gw, D)))
         ws, wp = _C.workspace(nbytes, x.device)
         st = L.mhc_linear_bwd(_C.ptr(xf), xs, _C.ptr(wf), wstr, _C.ptr(zf), zs, _C.ptr(gf), gs, T,
                               D, F, code, act, _C.ptr(gx), _C.ptr(gw), _C.ptr(gb), wp, nbytes,

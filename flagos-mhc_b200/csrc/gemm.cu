@@ -426,6 +426,8 @@ static GemmPlan gemm_plan(const Gemm& g) {
   return best;
 }
 
+bool gemm_few_form(const Gemm& g) { return gemm_plan(g).mt == 0; }
+
 size_t gemm_ws_bytes(const Gemm& g) {
   const GemmPlan p = gemm_plan(g);
   if (p.splits == 1 || p.mt == 0) return 0;
@@ -560,7 +562,8 @@ __global__ void __launch_bounds__(256)
 
 int pack_rows(const void* src, int64_t ls, int64_t rows, int64_t cols, void* dst, int64_t ld,
               cudaStream_t s) {
-  const bool four = (reinterpret_cast<uintptr_t>(src) & 3) == 0 && ls % 2 == 0 && cols % 2 == 0;
+  const bool four = ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 3) == 0 &&
+                    ls % 2 == 0 && ld % 2 == 0 && cols % 2 == 0;
   const dim3 grid((unsigned)std::min<int64_t>(cdiv(cols * 2, 256 * (four ? 4 : 2)), 64),
                   (unsigned)std::min<int64_t>(rows, 16384));
   if (four)

@@ -56,6 +56,7 @@ struct Gemm {
 // sizes alone (and whether a is K-major).
 size_t gemm_ws_bytes(const Gemm& g);
 int gemm_run(const Gemm& g, void* ws, cudaStream_t s);
+bool gemm_few_form(const Gemm& g);  // it takes the form of gemm_few.cu
 
 // The form with swapped roles (gemm_few.cu): its estimated time, tile and cut, and the run.
 double few_estimate(const Gemm& g, int* nt, int* splits);

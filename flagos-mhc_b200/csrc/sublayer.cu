@@ -155,7 +155,9 @@ struct Carver {
 };
 
 // An operand as the matrix product takes it: itself, or a packed copy in the workspace.
-static int64_t packed_bytes(int64_t rows, int64_t cols) { return rows * pad8(cols) * 2; }
+static size_t packed_bytes(int64_t rows, int64_t cols) {
+  return (size_t)rows * pad8(cols) * 2;
+}
 static int aligned_operand(Operand* o, int64_t rows, int64_t cols, Carver* c, cudaStream_t s) {
   if (operand_aligned(*o)) return MHC_OK;
   void* dst = c->take(packed_bytes(rows, cols));
@@ -192,6 +194,24 @@ static size_t ffn_bwd_room(int64_t T, int64_t D, int64_t F) {
                                  product(kEpiLinear, false, F, D, T), product(kEpiLinear, false, D, F, T)});
 }
 
+// Runs a product whose output's rows may be unaligned: then it goes to a packed copy first, for
+// the epilogue's row-wise stores (2 bytes to a row at a time: 2503 x 1001 outputs took 50 us, 27
+// us by the copy).  The copy's room is taken from the Carver and free again afterwards.
+static int run_product(Gemm* g, void* room, Carver c, cudaStream_t s) {
+  EpiParams& e = g->epi;
+  if (gemm_few_form(*g) || operand_aligned({e.out, e.ld_out, true})) return gemm_run(*g, room, s);
+  void *out = e.out, *z = e.z;
+  const int64_t ld = e.ld_out;
+  e.out = c.take(packed_bytes(g->M, g->N));
+  if (z) e.z = c.take(packed_bytes(g->M, g->N));
+  e.ld_out = pad8(g->N);
+  int st = gemm_run(*g, room, s);
+  if (st == MHC_OK) st = pack_rows(e.out, e.ld_out, g->M, g->N, out, ld, s);
+  if (st == MHC_OK && z) st = pack_rows(e.z, e.ld_out, g->M, g->N, z, ld, s);
+  e.out = out; e.z = z; e.ld_out = ld;
+  return st;
+}
+
 static bool any_unaligned(std::initializer_list<Operand> ops) {
   for (const Operand& o : ops)
     if (!operand_aligned(o)) return true;
@@ -223,6 +243,7 @@ size_t mhc_linear_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t d
   if (unaligned && !gemv_takes(T, F, D)) {
     c.take(packed_bytes(T, D));  // x
     c.take(packed_bytes(F, D));  // weight
+    for (int i = 0; i < 3; ++i) c.take(packed_bytes(T, F));  // residual, y, z
   }
   return c.off;
 }
@@ -242,7 +263,9 @@ int mhc_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   g.a = {x, x_stride, true};
   g.b = {weight, weight_stride, true};
   if (!ws_ok(workspace, workspace_bytes,
-             mhc_linear_fwd_workspace_bytes(T, D, F, dtype, any_unaligned({g.a, g.b}))))
+             mhc_linear_fwd_workspace_bytes(
+                 T, D, F, dtype,
+                 any_unaligned({g.a, g.b, {y, F, true}, {residual, residual_stride, true}}))))
     return MHC_ERR_WORKSPACE;
   RETURN_IF(check_device());
   const cudaStream_t s = (cudaStream_t)stream;
@@ -253,7 +276,12 @@ int mhc_linear_fwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   if (gemv_takes(T, F, D)) return gemv_run(g, s);
   RETURN_IF(aligned_operand(&g.a, T, D, &c, s));
   RETURN_IF(aligned_operand(&g.b, F, D, &c, s));
-  return gemm_run(g, room, s);
+  if (residual) {
+    Operand r{residual, residual_stride, true};
+    RETURN_IF(aligned_operand(&r, T, F, &c, s));
+    g.epi.res = r.p; g.epi.ld_res = r.ld;
+  }
+  return run_product(&g, room, c, s);
 }
 
 size_t mhc_linear_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
@@ -264,8 +292,9 @@ size_t mhc_linear_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t d
   c.take((size_t)gz_ranges(T, F) * F * 4);
   c.take(linear_bwd_room(T, D, F));
   if (unaligned) {
-    c.take(packed_bytes(T, D));  // x
-    c.take(packed_bytes(F, D));  // weight
+    c.take(packed_bytes(T, D));                               // x
+    c.take(packed_bytes(F, D));                               // weight
+    c.take(std::max(packed_bytes(T, D), packed_bytes(F, D)));  // grad_x, then grad_weight
   }
   return c.off;
 }
@@ -286,7 +315,7 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   const bool gy_packed = act == MHC_ACT_NONE && !operand_aligned({grad_y, grad_y_stride, false});
   if (T > 0 && !ws_ok(workspace, workspace_bytes,
                       mhc_linear_bwd_workspace_bytes(T, D, F, dtype, act,
-                                                     gy_packed || any_unaligned({ox, ow}))))
+                                                     gy_packed || any_unaligned({ox, ow, {grad_x, D, true}, {grad_weight, D, true}}))))
     return MHC_ERR_WORKSPACE;
   RETURN_IF(check_device());
   if (T == 0) {
@@ -308,23 +337,23 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   }
   const void* gz = gzb ? gzb : grad_y;
   const int64_t gzs = gzb ? pad8(F) : grad_y_stride;
+  if (grad_x) RETURN_IF(aligned_operand(&ow, F, D, &c, s));
+  if (grad_weight) RETURN_IF(aligned_operand(&ox, T, D, &c, s));
   Gemm g;
   g.dtype = dtype;
   if (grad_x) {
-    RETURN_IF(aligned_operand(&ow, F, D, &c, s));
     g.M = T; g.N = D; g.K = F;
     g.a = {gz, gzs, true};
     g.b = ow;
     g.epi.out = grad_x; g.epi.ld_out = D;
-    RETURN_IF(gemm_run(g, room, s));
+    RETURN_IF(run_product(&g, room, c, s));
   }
   if (grad_weight) {
-    RETURN_IF(aligned_operand(&ox, T, D, &c, s));
     g.M = F; g.N = D; g.K = T;
     g.a = {gz, gzs, false};
     g.b = ox;
     g.epi.out = grad_weight; g.epi.ld_out = D;
-    RETURN_IF(gemm_run(g, room, s));
+    RETURN_IF(run_product(&g, room, c, s));
   }
   return MHC_OK;
 }
@@ -339,6 +368,7 @@ size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_
     c.take(packed_bytes(T, D));                              // x
     for (int i = 0; i < 2; ++i) c.take(packed_bytes(F, D));  // w_gate, w_up
     c.take(packed_bytes(D, F));                              // w_down
+    c.take(packed_bytes(T, D));                              // y
   }
   return c.off;
 }
@@ -357,7 +387,8 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   Operand ox{x, x_stride, true}, og{w_gate, w_gate_stride, true}, ou{w_up, w_up_stride, true},
       od{w_down, w_down_stride, true};
   if (!ws_ok(workspace, workspace_bytes,
-             mhc_gated_ffn_fwd_workspace_bytes(T, D, F, dtype, any_unaligned({ox, og, ou, od}))))
+             mhc_gated_ffn_fwd_workspace_bytes(
+                 T, D, F, dtype, any_unaligned({ox, og, ou, od, {y, D, true}}))))
     return MHC_ERR_WORKSPACE;
   RETURN_IF(check_device());
   const cudaStream_t s = (cudaStream_t)stream;
@@ -388,7 +419,7 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   d.a = {h, ldh, true};
   d.b = od;
   d.epi.out = y; d.epi.ld_out = D;
-  return few ? gemv_run(d, s) : gemm_run(d, room, s);
+  return few ? gemv_run(d, s) : run_product(&d, room, c, s);
 }
 
 size_t mhc_gated_ffn_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
@@ -401,6 +432,7 @@ size_t mhc_gated_ffn_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_
     for (int i = 0; i < 2; ++i) c.take(packed_bytes(T, D));  // x, grad_y
     for (int i = 0; i < 2; ++i) c.take(packed_bytes(F, D));  // w_gate, w_up
     c.take(packed_bytes(D, F));                              // w_down
+    c.take(std::max(packed_bytes(T, D), std::max(packed_bytes(F, D), packed_bytes(D, F))));
   }
   return c.off;
 }
@@ -424,7 +456,10 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
       od{w_down, w_down_stride, false};
   if (T > 0 &&
       !ws_ok(workspace, workspace_bytes,
-             mhc_gated_ffn_bwd_workspace_bytes(T, D, F, dtype, any_unaligned({ox, oy, og, ou, od}))))
+             mhc_gated_ffn_bwd_workspace_bytes(
+                 T, D, F, dtype,
+                 any_unaligned({ox, oy, og, ou, od, {grad_x, D, true}, {grad_w_gate, D, true},
+                                {grad_w_up, D, true}, {grad_w_down, F, true}}))))
     return MHC_ERR_WORKSPACE;
   RETURN_IF(check_device());
   if (T == 0) {
@@ -454,11 +489,14 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
     g.epi.out = h; g.epi.ld_out = ld;
     RETURN_IF(gemm_run(g, room, s));
   }
-  Gemm g;
-  g.dtype = dtype;
   if (grad_x) {
     RETURN_IF(aligned_operand(&og, F, D, &c, s));
     RETURN_IF(aligned_operand(&ou, F, D, &c, s));
+  }
+  if (grad_w_gate || grad_w_up) RETURN_IF(aligned_operand(&ox, T, D, &c, s));
+  Gemm g;
+  g.dtype = dtype;
+  if (grad_x) {
     g.M = T; g.N = D; g.K = F;
     g.a = {gg, ld, true};
     g.b = og;
@@ -466,10 +504,9 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
     g.b3 = ou;
     g.K3 = F;
     g.epi.out = grad_x; g.epi.ld_out = D;
-    RETURN_IF(gemm_run(g, room, s));
+    RETURN_IF(run_product(&g, room, c, s));
     g.K3 = 0;
   }
-  if (grad_w_gate || grad_w_up) RETURN_IF(aligned_operand(&ox, T, D, &c, s));
   g.K = T;
   g.M = F; g.N = D;
   g.b = ox;
@@ -477,19 +514,19 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
   if (grad_w_gate) {
     g.a = {gg, ld, false};
     g.epi.out = grad_w_gate;
-    RETURN_IF(gemm_run(g, room, s));
+    RETURN_IF(run_product(&g, room, c, s));
   }
   if (grad_w_up) {
     g.a = {gu, ld, false};
     g.epi.out = grad_w_up;
-    RETURN_IF(gemm_run(g, room, s));
+    RETURN_IF(run_product(&g, room, c, s));
   }
   if (grad_w_down) {
     g.M = D; g.N = F;
     g.a = {oy.p, oy.ld, false};
     g.b = {h, ld, false};
     g.epi.out = grad_w_down; g.epi.ld_out = F;
-    RETURN_IF(gemm_run(g, room, s));
+    RETURN_IF(run_product(&g, room, c, s));
   }
   return MHC_OK;
 }

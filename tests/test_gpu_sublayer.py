@@ -186,7 +186,7 @@ def test_layer_norm_special_rows():
 LIN_SHAPES = [(1, 1, 1), (1, 8, 8), (2, 5, 7), (3, 64, 200), (17, 72, 40), (9, 520, 1000),
               (33, 1000, 264), (64, 256, 512), (65, 129, 255), (130, 264, 136), (257, 328, 513),
               (300, 1024, 640), (513, 2048, 256), (1, 4096, 1032), (8, 3000, 2048),
-              (48, 1536, 768)]
+              (48, 1536, 768), (1100, 257, 515), (2100, 1030, 771)]
 
 
 def lin_case(T, D, F, dt, seed):
@@ -327,7 +327,7 @@ def test_rows_keep_to_themselves():
 # ------------------------------------------------------------------ gated feed-forward
 FFN_SHAPES = [(1, 1, 1), (1, 64, 72), (2, 7, 5), (5, 200, 136), (16, 512, 1000), (33, 264, 520),
               (64, 1024, 512), (65, 100, 255), (140, 328, 264), (257, 136, 1023), (300, 512, 384),
-              (3, 4096, 640), (48, 768, 2048)]
+              (3, 4096, 640), (48, 768, 2048), (1100, 257, 131), (1300, 520, 1290)]
 
 
 def ffn_case(T, D, F, dt, seed):
