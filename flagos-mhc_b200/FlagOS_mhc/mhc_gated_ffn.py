@@ -48,7 +48,7 @@ def mhc_gated_ffn(x, w_gate, w_up, w_down, activation="silu", need_backward=Fals
     dev = x.device
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     gate = up = None
-    ld = (F + 7) // 8 * 8  # rows start on 16-byte boundaries
+    ld = (F + 15) // 16 * 16  # rows start on 32-byte boundaries
     if need_backward:
         gate, up = torch.empty(2, T, ld, dtype=x.dtype, device=dev)[:, :, :F].unbind(0)
     L = _C.lib()

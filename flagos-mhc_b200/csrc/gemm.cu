@@ -315,11 +315,25 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
     for (int32_t i = first; i < units; i += step, ++j) {
       const Unit u = unit_at<MT>(w, i);
       const uint32_t buf = MT == 1 ? j & 1 : pair, ph = MT == 1 ? (j >> 1) & 1 : j & 1;
+      const int64_t row = (int64_t)u.mt * ROWS + (MT == 1 ? 0 : pair * 256) + rank * BM + q * 32 + lane;
+      const int64_t col0 = (int64_t)u.nt * (dual ? BNC : 2 * BNC) + col_off;
+      // kEpiGatedBwd reads gate and up: a chunk ahead, the first before the products are done
+      constexpr bool ahead = KIND == kEpiGatedBwd;
+      Raw32 pre[ahead ? 4 : 1];
+      auto fetch = [&](int c) {
+        if constexpr (ahead) {
+          if (row < w.M && epi.vec == 2 && w.splits == 1 && col0 + c + 32 <= w.N) {
+            const E* pg = reinterpret_cast<const E*>(epi.gate) + row * epi.ld_gu + col0 + c;
+            const E* pu = reinterpret_cast<const E*>(epi.up) + row * epi.ld_gu + col0 + c;
+            pre[0] = ld_row32(pg); pre[1] = ld_row32(pg + 16);
+            pre[2] = ld_row32(pu); pre[3] = ld_row32(pu + 16);
+          }
+        }
+      };
+      fetch(0);
       const bool got = tc::mbar_wait(&tfull[buf], ph, abort_flag);
       if (!__all_sync(0xffffffffu, got)) break;
       tc::tc_fence_after();
-      const int64_t row = (int64_t)u.mt * ROWS + (MT == 1 ? 0 : pair * 256) + rank * BM + q * 32 + lane;
-      const int64_t col0 = (int64_t)u.nt * (dual ? BNC : 2 * BNC) + col_off;
 #pragma unroll 1
       for (int c = 0; c < COLS; c += 32) {
         __syncwarp();  // rows past M skip the epilogue below
@@ -335,7 +349,23 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
         const int64_t left = w.N - (col0 + c);
         if (row < w.M && left > 0) {
           if (w.splits == 1) {
-            epi_chunk<E, KIND, 32>(epi, row, col0 + c, left < 32 ? (int)left : 32, acc, acc2);
+            if constexpr (ahead) {
+              if (epi.vec == 2 && left >= 32) {
+                float gu[64];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  widen<E>(pre[k].a, gu + 16 * k);
+                  widen<E>(pre[k].b, gu + 16 * k + 8);
+                }
+                if (c + 32 < COLS) fetch(c + 32);
+                epi_chunk<E, KIND, 32>(epi, row, col0 + c, 32, acc, gu);
+              } else {
+                epi_chunk<E, KIND, 32>(epi, row, col0 + c, left < 32 ? (int)left : 32, acc, nullptr);
+              }
+            } else {
+              epi_chunk<E, KIND, 32>(epi, row, col0 + c, left < 32 ? (int)left : 32, acc,
+                                     dual ? acc2 : nullptr);
+            }
           } else {  // ldp is N rounded up to 32
             float* d = w.part + ((int64_t)u.split * (dual ? 2 : 1) * w.M + row) * w.ldp + col0 + c;
 #pragma unroll
@@ -384,7 +414,8 @@ __global__ void __launch_bounds__(256)
         acc[p][4] += b.x; acc[p][5] += b.y; acc[p][6] += b.z; acc[p][7] += b.w;
       }
     }
-    epi_chunk<E, KIND, 8>(epi, row, col, N - col < 8 ? (int)(N - col) : 8, acc[0], acc[PL - 1]);
+    epi_chunk<E, KIND, 8>(epi, row, col, N - col < 8 ? (int)(N - col) : 8, acc[0],
+                          PL == 2 ? acc[PL - 1] : nullptr);
   }
 }
 
@@ -434,11 +465,13 @@ size_t gemm_ws_bytes(const Gemm& g) {
   return align_up((size_t)p.splits * (g.kind == kEpiGated ? 2 : 1) * g.M * part_ld(g) * 4);
 }
 
-bool epi_vec_ok(const Gemm& g) {
-  const EpiParams& e = g.epi;
-  return aligned16(e.out) && e.ld_out % 8 == 0 && aligned16(e.bias) && aligned16(e.res) &&
-         e.ld_res % 8 == 0 && aligned16(e.z) && aligned16(e.gate) && aligned16(e.up) &&
-         e.ld_gu % 8 == 0 && aligned16(e.gg) && aligned16(e.gu) && e.ld_g % 8 == 0;
+int epi_vec(const EpiParams& e) {
+  uintptr_t bits = 0;
+  for (const void* p : {(const void*)e.out, e.bias, e.res, (const void*)e.z, (const void*)e.gate,
+                        (const void*)e.up, (const void*)e.gg, (const void*)e.gu})
+    bits |= reinterpret_cast<uintptr_t>(p);
+  for (int64_t ld : {e.ld_out, e.ld_res, e.ld_gu, e.ld_g}) bits |= (uintptr_t)ld * 2;
+  return (bits & 31) == 0 ? 2 : (bits & 15) == 0 ? 1 : 0;
 }
 
 bool operand_aligned(const Operand& o) { return aligned16(o.p) && o.ld % 8 == 0; }
@@ -536,7 +569,7 @@ static int gemm_typed(const Gemm& g, void* ws, cudaStream_t s) {
 
 int gemm_run(const Gemm& g0, void* ws, cudaStream_t s) {
   Gemm g = g0;
-  g.epi.vec = epi_vec_ok(g);
+  g.epi.vec = epi_vec(g.epi);
   return g.dtype == MHC_F16 ? gemm_typed<__half>(g, ws, s) : gemm_typed<__nv_bfloat16>(g, ws, s);
 }
 

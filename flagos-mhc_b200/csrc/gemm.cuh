@@ -38,7 +38,7 @@ struct EpiParams {
   void* gg = nullptr;
   void* gu = nullptr;
   int64_t ld_g = 0;
-  bool vec = false;  // every row above starts on a 16-byte boundary
+  int vec = 0;  // 1: every row above starts on a 16-byte boundary, 2: on a 32-byte one
 };
 
 struct Gemm {
@@ -72,14 +72,40 @@ bool operand_aligned(const Operand& o);
 int pack_rows(const void* src, int64_t ls, int64_t rows, int64_t cols, void* dst, int64_t ld,
               cudaStream_t s);
 
-// Whether all rows the epilogue touches start on 16-byte boundaries.
-bool epi_vec_ok(const Gemm& g);
+// EpiParams::vec
+int epi_vec(const EpiParams& e);
 
 // ---------------------------------------------------------------- epilogue
+// A thread owns a row here, so every access of a warp touches 32 rows: 32-byte accesses (whole
+// sectors) halve the requests where the rows allow them.
+struct alignas(32) Raw32 {
+  uint4 a, b;
+};
+__device__ __forceinline__ Raw32 ld_row32(const void* p) {
+  Raw32 v;
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v.a.x), "=r"(v.a.y), "=r"(v.a.z), "=r"(v.a.w), "=r"(v.b.x), "=r"(v.b.y),
+                 "=r"(v.b.z), "=r"(v.b.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_row32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y),
+               "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
 template <typename E, int NC>
-__device__ __forceinline__ void row_load(const void* base, int64_t off, int n, bool vec, float* f) {
+__device__ __forceinline__ void row_load(const void* base, int64_t off, int n, int vec, float* f) {
   const E* p = reinterpret_cast<const E*>(base) + off;
-  if (vec && n == NC) {
+  if (NC % 16 == 0 && vec == 2 && n == NC) {
+#pragma unroll
+    for (int i = 0; i < NC; i += 16) {
+      const Raw32 r = ld_row32(p + i);
+      widen<E>(r.a, f + i);
+      widen<E>(r.b, f + i + 8);
+    }
+  } else if (NC % 8 == 0 && vec && n == NC) {
 #pragma unroll
     for (int i = 0; i < NC; i += 8) widen<E>(*reinterpret_cast<const uint4*>(p + i), f + i);
   } else {
@@ -88,9 +114,12 @@ __device__ __forceinline__ void row_load(const void* base, int64_t off, int n, b
   }
 }
 template <typename E, int NC>
-__device__ __forceinline__ void row_store(void* base, int64_t off, int n, bool vec, const float* f) {
+__device__ __forceinline__ void row_store(void* base, int64_t off, int n, int vec, const float* f) {
   E* p = reinterpret_cast<E*>(base) + off;
-  if (vec && n == NC) {
+  if (NC % 16 == 0 && vec == 2 && n == NC) {
+#pragma unroll
+    for (int i = 0; i < NC; i += 16) st_row32(p + i, narrow<E>(f + i), narrow<E>(f + i + 8));
+  } else if (NC % 8 == 0 && vec && n == NC) {
 #pragma unroll
     for (int i = 0; i < NC; i += 8) *reinterpret_cast<uint4*>(p + i) = narrow<E>(f + i);
   } else {
@@ -101,7 +130,8 @@ __device__ __forceinline__ void row_store(void* base, int64_t off, int n, bool v
 }
 
 // n <= NC valid columns of one row, starting at col (a multiple of 8).  acc: the product;
-// acc2: the second product of kEpiGated.
+// acc2: the second product of kEpiGated; for kEpiGatedBwd gate and up where they were loaded
+// ahead, else null.
 template <typename E, int KIND, int ACT, int NC>
 __device__ __forceinline__ void epi_act(const EpiParams& e, int64_t row, int64_t col, int n,
                                         float* acc, const float* acc2) {
@@ -131,8 +161,13 @@ __device__ __forceinline__ void epi_act(const EpiParams& e, int64_t row, int64_t
     row_store<E, NC>(e.out, row * e.ld_out + col, n, e.vec, v);
   } else {
     float u[NC];
-    row_load<E, NC>(e.gate, row * e.ld_gu + col, n, e.vec, v);
-    row_load<E, NC>(e.up, row * e.ld_gu + col, n, e.vec, u);
+    if (acc2) {  // loaded ahead: gate in v's place, then up
+#pragma unroll
+      for (int i = 0; i < NC; ++i) v[i] = acc2[i], u[i] = acc2[NC + i];
+    } else {
+      row_load<E, NC>(e.gate, row * e.ld_gu + col, n, e.vec, v);
+      row_load<E, NC>(e.up, row * e.ld_gu + col, n, e.vec, u);
+    }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       float a, da;

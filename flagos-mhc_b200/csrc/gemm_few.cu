@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(fk::THREADS, 1)
         }
       }
     }
-    epi_chunk<E, KIND, 8>(epi, t0 + tok, f0 + f, left < 8 ? (int)left : 8, v[0], v[W - 1]);
+    epi_chunk<E, KIND, 8>(epi, t0 + tok, f0 + f, left < 8 ? (int)left : 8, v[0],
+                          W == 2 ? v[W - 1] : nullptr);
   }
   if (*abort_flag && threadIdx.x == 0) flag_timeout();
   if (w.splits > 1)

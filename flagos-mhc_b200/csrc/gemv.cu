@@ -181,7 +181,7 @@ bool gemv_takes(int64_t M, int64_t N, int64_t K) {
 
 int gemv_run(const Gemm& g0, cudaStream_t s) {
   Gemm g = g0;
-  g.epi.vec = false;  // element by element
+  g.epi.vec = 0;  // element by element
   return g.dtype == MHC_F16 ? gemv_typed<__half>(g, s) : gemv_typed<__nv_bfloat16>(g, s);
 }
 

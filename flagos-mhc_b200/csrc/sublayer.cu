@@ -128,7 +128,7 @@ static int act_bwd_run(int act, const void* z, int64_t zs, const void* gy, int64
 }
 
 // ------------------------------------------------------------------ checks and workspace
-static int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+static int64_t pad16(int64_t n) { return (n + 15) / 16 * 16; }  // rows on 32-byte boundaries
 
 static int sub_check(int64_t T, int64_t D, int64_t F, int32_t dtype, int32_t act) {
   // tile coordinates are 32-bit
@@ -156,14 +156,14 @@ struct Carver {
 
 // An operand as the matrix product takes it: itself, or a packed copy in the workspace.
 static size_t packed_bytes(int64_t rows, int64_t cols) {
-  return (size_t)rows * pad8(cols) * 2;
+  return (size_t)rows * pad16(cols) * 2;
 }
 static int aligned_operand(Operand* o, int64_t rows, int64_t cols, Carver* c, cudaStream_t s) {
   if (operand_aligned(*o)) return MHC_OK;
   void* dst = c->take(packed_bytes(rows, cols));
-  const int st = pack_rows(o->p, o->ld, rows, cols, dst, pad8(cols), s);
+  const int st = pack_rows(o->p, o->ld, rows, cols, dst, pad16(cols), s);
   o->p = dst;
-  o->ld = pad8(cols);
+  o->ld = pad16(cols);
   return st;
 }
 // Room for the partial products of the largest of these products (they run one by one).
@@ -204,7 +204,7 @@ static int run_product(Gemm* g, void* room, Carver c, cudaStream_t s) {
   const int64_t ld = e.ld_out;
   e.out = c.take(packed_bytes(g->M, g->N));
   if (z) e.z = c.take(packed_bytes(g->M, g->N));
-  e.ld_out = pad8(g->N);
+  e.ld_out = pad16(g->N);
   int st = gemm_run(*g, room, s);
   if (st == MHC_OK) st = pack_rows(e.out, e.ld_out, g->M, g->N, out, ld, s);
   if (st == MHC_OK && z) st = pack_rows(e.z, e.ld_out, g->M, g->N, z, ld, s);
@@ -328,7 +328,7 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   float* part = (float*)c.take((size_t)gz_ranges(T, F) * F * 4);
   void* room = c.take(linear_bwd_room(T, D, F));
   if (gzb || grad_bias) {
-    const int64_t ld = pad8(F);
+    const int64_t ld = pad16(F);
     RETURN_IF(dtype == MHC_F16
                   ? act_bwd_run<__half>(act, z, z_stride, grad_y, grad_y_stride, T, F, gzb, ld,
                                         grad_bias, part, s)
@@ -336,7 +336,7 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
                                                ld, grad_bias, part, s));
   }
   const void* gz = gzb ? gzb : grad_y;
-  const int64_t gzs = gzb ? pad8(F) : grad_y_stride;
+  const int64_t gzs = gzb ? pad16(F) : grad_y_stride;
   if (grad_x) RETURN_IF(aligned_operand(&ow, F, D, &c, s));
   if (grad_weight) RETURN_IF(aligned_operand(&ox, T, D, &c, s));
   Gemm g;
@@ -393,7 +393,7 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   RETURN_IF(check_device());
   const cudaStream_t s = (cudaStream_t)stream;
   Carver c{(char*)workspace};
-  const int64_t ldh = pad8(F);
+  const int64_t ldh = pad16(F);
   void* h = c.take(packed_bytes(T, F));
   void* room = c.take(ffn_fwd_room(T, D, F));
   const bool few = gemv_takes(T, F, D);
@@ -468,7 +468,7 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
     return zero(grad_w_down, (size_t)F * D * 2, s);
   }
   Carver c{(char*)workspace};
-  const int64_t ld = pad8(F);
+  const int64_t ld = pad16(F);
   void* gg = c.take(packed_bytes(T, F));
   void* gu = c.take(packed_bytes(T, F));
   void* h = c.take(packed_bytes(T, F));
