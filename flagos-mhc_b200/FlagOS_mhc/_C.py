@@ -160,6 +160,11 @@ def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def addr(t):
+    """The same as a plain integer (cheaper to make; ctypes converts it)."""
+    return None if t is None else t.data_ptr()
+
+
 def dtype_code(dt):
     try:
         return _DTYPE[dt]
@@ -173,9 +178,13 @@ _no_guard = contextlib.nullcontext()
 
 
 def stream_of(t):
+    return ctypes.c_void_p(stream_addr(t.device))
+
+
+def stream_addr(device):
     if _raw_stream is not None:
-        return ctypes.c_void_p(_raw_stream(t.device.index))
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def device_guard(device):
@@ -206,13 +215,14 @@ def require_cuda(*tensors):
 
 def require_same(what, x, *others):
     """The other tensors of a call: x's device and dtype (None is skipped)."""
+    device, dtype = x.device, x.dtype
     for t in others:
         if t is None:
             continue
-        if t.device != x.device:
-            raise RuntimeError(f"FlagOS_mhc.{what}: tensors on {x.device} and {t.device}")
-        if t.dtype != x.dtype:
-            raise ValueError(f"FlagOS_mhc.{what}: dtypes {x.dtype} and {t.dtype} in one call")
+        if t.device != device:
+            raise RuntimeError(f"FlagOS_mhc.{what}: tensors on {device} and {t.device}")
+        if t.dtype != dtype:
+            raise ValueError(f"FlagOS_mhc.{what}: dtypes {dtype} and {t.dtype} in one call")
 
 
 def act_code(name):
@@ -248,4 +258,4 @@ def workspace(nbytes, device):
     if nbytes == 0:
         return None, None
     t = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return t, ptr(t)
+    return t, t.data_ptr()

@@ -46,7 +46,7 @@ def mhc_gated_ffn(x, w_gate, w_up, w_down, activation="silu", need_backward=Fals
     uf, us = _C.rows(w_up, D)
     df, ds = _C.rows(w_down, F)
     dev = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     gate = up = None
     ld = (F + 15) // 16 * 16  # rows start on 32-byte boundaries
     if need_backward:
@@ -56,9 +56,9 @@ def mhc_gated_ffn(x, w_gate, w_up, w_down, activation="silu", need_backward=Fals
         nbytes = L.mhc_gated_ffn_fwd_workspace_bytes(
             T, D, F, code, _C.unaligned((xf, xs), (gf, gs), (uf, us), (df, ds), (y, D)))
         ws, wp = _C.workspace(nbytes, dev)
-        st = L.mhc_gated_ffn_fwd(_C.ptr(xf), xs, _C.ptr(gf), gs, _C.ptr(uf), us, _C.ptr(df), ds, T,
-                                 D, F, code, act, _C.ptr(y), _C.ptr(gate), _C.ptr(up), ld, wp,
-                                 nbytes, _C.stream_of(x))
+        st = L.mhc_gated_ffn_fwd(_C.addr(xf), xs, _C.addr(gf), gs, _C.addr(uf), us, _C.addr(df), ds, T,
+                                 D, F, code, act, _C.addr(y), _C.addr(gate), _C.addr(up), ld, wp,
+                                 nbytes, _C.stream_addr(x.device))
     _C.check(st, "mhc_gated_ffn")
     return {"y": y, "gate": gate, "up": up} if need_backward else {"y": y}
 

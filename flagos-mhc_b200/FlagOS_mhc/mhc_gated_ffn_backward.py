@@ -42,9 +42,9 @@ def mhc_gated_ffn_backward(x, w_gate, w_up, w_down, gate, up, grad_y, activation
         nbytes = L.mhc_gated_ffn_bwd_workspace_bytes(
             T, D, F, code, _C.unaligned((xf, xs), (wg, wgs), (wu, wus), (wd, wds), (gf, gs), (wg, D), (wd, F)))
         ws, wp = _C.workspace(nbytes, x.device)
-        st = L.mhc_gated_ffn_bwd(_C.ptr(xf), xs, _C.ptr(wg), wgs, _C.ptr(wu), wus, _C.ptr(wd), wds,
-                                 _C.ptr(ga), _C.ptr(ua), gas, _C.ptr(gf), gs, T, D, F, code, act,
-                                 *(_C.ptr(o) for o in outs), wp, nbytes, _C.stream_of(x))
+        st = L.mhc_gated_ffn_bwd(_C.addr(xf), xs, _C.addr(wg), wgs, _C.addr(wu), wus, _C.addr(wd), wds,
+                                 _C.addr(ga), _C.addr(ua), gas, _C.addr(gf), gs, T, D, F, code, act,
+                                 *(_C.addr(o) for o in outs), wp, nbytes, _C.stream_addr(x.device))
     _C.check(st, "mhc_gated_ffn_backward")
     return tuple(outs)
 

@@ -18,7 +18,7 @@ def _check_params(x, weight, bias):
         raise ValueError("mhc_layer_norm: rows of width 0")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None:
-            assert tuple(p.shape) == (D,), f"{name} shape {tuple(p.shape)} != {(D,)}"
+            assert p.dim() == 1 and p.numel() == D, f"{name} shape {tuple(p.shape)} != {(D,)}"
             if p.device != x.device:
                 raise RuntimeError(f"FlagOS_mhc.mhc_layer_norm: tensors on {x.device} and "
                                    f"{p.device}")
@@ -50,15 +50,15 @@ def mhc_layer_norm(x, weight=None, bias=None, eps=1e-5, need_backward=False):
     xf, xs = _C.rows(x, D)
     w, b = _param(weight), _param(bias)
     dev = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = None
     if need_backward:
         mean = torch.empty(T, dtype=torch.float32, device=dev)
         rstd = torch.empty(T, dtype=torch.float32, device=dev)
     with _C.device_guard(dev):
-        st = _C.lib().mhc_layer_norm_fwd(_C.ptr(xf), xs, _C.ptr(w), _C.ptr(b), T, D, code,
-                                         float(eps), _C.ptr(y), _C.ptr(mean), _C.ptr(rstd),
-                                         _C.stream_of(x))
+        st = _C.lib().mhc_layer_norm_fwd(_C.addr(xf), xs, _C.addr(w), _C.addr(b), T, D, code,
+                                         float(eps), _C.addr(y), _C.addr(mean), _C.addr(rstd),
+                                         _C.stream_addr(x.device))
     _C.check(st, "mhc_layer_norm")
     return {"y": y, "mean": mean, "rstd": rstd} if need_backward else {"y": y}
 

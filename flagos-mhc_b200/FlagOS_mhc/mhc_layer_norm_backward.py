@@ -31,7 +31,7 @@ def mhc_layer_norm_backward(x, weight, mean, rstd, grad_y, need_param_grads=True
     gf, gs = _C.rows(grad_y, D)
     w, m, r = _param(weight), _param(mean), _param(rstd)
     dev = x.device
-    grad_x = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    grad_x = torch.empty_like(x, memory_format=torch.contiguous_format)
     gw = gb = ws = wp = None
     nbytes = 0
     L = _C.lib()
@@ -40,9 +40,9 @@ def mhc_layer_norm_backward(x, weight, mean, rstd, grad_y, need_param_grads=True
             gw, gb = torch.empty(2, D, dtype=torch.float32, device=dev).unbind(0)
             nbytes = L.mhc_layer_norm_bwd_workspace_bytes(T, D, code)
             ws, wp = _C.workspace(nbytes, dev)
-        st = L.mhc_layer_norm_bwd(_C.ptr(xf), xs, _C.ptr(w), _C.ptr(m), _C.ptr(r), _C.ptr(gf), gs,
-                                  T, D, code, _C.ptr(grad_x), _C.ptr(gw), _C.ptr(gb), wp, nbytes,
-                                  _C.stream_of(x))
+        st = L.mhc_layer_norm_bwd(_C.addr(xf), xs, _C.addr(w), _C.addr(m), _C.addr(r), _C.addr(gf), gs,
+                                  T, D, code, _C.addr(grad_x), _C.addr(gw), _C.addr(gb), wp, nbytes,
+                                  _C.stream_addr(x.device))
     _C.check(st, "mhc_layer_norm_backward")
     return grad_x, gw, gb
 

@@ -62,8 +62,8 @@ def mhc_linear(x, weight, bias=None, residual=None, activation="none", need_back
         nbytes = L.mhc_linear_fwd_workspace_bytes(T, D, F, code,
                                                   _C.unaligned((xf, xs), (wf, wstr), (rf, rs), (y, F)))
         ws, wp = _C.workspace(nbytes, dev)
-        st = L.mhc_linear_fwd(_C.ptr(xf), xs, _C.ptr(wf), wstr, _C.ptr(bf), _C.ptr(rf), rs, T, D,
-                              F, code, act, _C.ptr(y), _C.ptr(z), wp, nbytes, _C.stream_of(x))
+        st = L.mhc_linear_fwd(_C.addr(xf), xs, _C.addr(wf), wstr, _C.addr(bf), _C.addr(rf), rs, T, D,
+                              F, code, act, _C.addr(y), _C.addr(z), wp, nbytes, _C.stream_addr(x.device))
     _C.check(st, "mhc_linear")
     return {"y": y, "z": z} if need_backward else {"y": y}
 

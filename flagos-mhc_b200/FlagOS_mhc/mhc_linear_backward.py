@@ -42,9 +42,9 @@ def mhc_linear_backward(x, weight, z, grad_y, activation="none", need_x_grad=Tru
         nbytes = L.mhc_linear_bwd_workspace_bytes(
             T, D, F, code, act, _C.unaligned((xf, xs), (wf, wstr), (gf, gs), (gx, D), (gw, D)))
         ws, wp = _C.workspace(nbytes, x.device)
-        st = L.mhc_linear_bwd(_C.ptr(xf), xs, _C.ptr(wf), wstr, _C.ptr(zf), zs, _C.ptr(gf), gs, T,
-                              D, F, code, act, _C.ptr(gx), _C.ptr(gw), _C.ptr(gb), wp, nbytes,
-                              _C.stream_of(x))
+        st = L.mhc_linear_bwd(_C.addr(xf), xs, _C.addr(wf), wstr, _C.addr(zf), zs, _C.addr(gf), gs, T,
+                              D, F, code, act, _C.addr(gx), _C.addr(gw), _C.addr(gb), wp, nbytes,
+                              _C.stream_addr(x.device))
     _C.check(st, "mhc_linear_backward")
     return gx, gw, gb
 

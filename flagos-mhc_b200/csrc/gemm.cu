@@ -447,7 +447,8 @@ static GemmPlan gemm_plan(const Gemm& g) {
     const double per_k = mt == 1 ? 0.40 : 0.75;
     const double tail = mt == 1 ? 1.0 : g.kind == kEpiLinear ? 2.0 : dual ? 3.0 : 20.0;
     for (int sp = 1; sp <= 16; ++sp) {
-      if (sp > 1 && (nk < 4 * sp || plane * sp * 4 > 1e9)) break;
+      // (beyond eight waves a cut gains nothing)
+      if (sp > 1 && (nk < 4 * sp || plane * sp * 4 > 1e9 || tiles * (sp - 1) > 8 * clusters)) break;
       const double waves = (double)cdiv(tiles * sp, clusters);
       double us = 7.0 + waves * ((double)cdiv(nk, sp) * per_k + tail);
       if (sp > 1) us += 3.0 + plane * sp * 8 / 4e6;
