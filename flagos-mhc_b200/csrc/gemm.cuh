@@ -129,12 +129,21 @@ __device__ __forceinline__ void row_store(void* base, int64_t off, int n, int ve
   }
 }
 
+// Where an epilogue's outputs go: which = 0: out, 1: z, gate or gg, 2: up or gu.
+struct StoreRows {
+  template <typename E, int NC>
+  __device__ __forceinline__ void put(int which, void* base, int64_t row, int64_t ld, int64_t col,
+                                      int n, int vec, const float* f) const {
+    row_store<E, NC>(base, row * ld + col, n, vec, f);
+  }
+};
+
 // n <= NC valid columns of one row, starting at col (a multiple of 8).  acc: the product;
 // acc2: the second product of kEpiGated; for kEpiGatedBwd gate and up where they were loaded
 // ahead, else null.
-template <typename E, int KIND, int ACT, int NC>
+template <typename E, int KIND, int ACT, int NC, typename Store>
 __device__ __forceinline__ void epi_act(const EpiParams& e, int64_t row, int64_t col, int n,
-                                        float* acc, const float* acc2) {
+                                        float* acc, const float* acc2, Store& st) {
   float v[NC];
   if constexpr (KIND == kEpiLinear) {
     if (e.bias) {
@@ -142,7 +151,7 @@ __device__ __forceinline__ void epi_act(const EpiParams& e, int64_t row, int64_t
 #pragma unroll
       for (int i = 0; i < NC; ++i) acc[i] += v[i];
     }
-    if (e.z) row_store<E, NC>(e.z, row * e.ld_out + col, n, e.vec, acc);
+    if (e.z) st.template put<E, NC>(1, e.z, row, e.ld_out, col, n, e.vec, acc);
 #pragma unroll
     for (int i = 0; i < NC; ++i) acc[i] = act_fwd<ACT>(acc[i]);
     if (e.res) {
@@ -150,15 +159,15 @@ __device__ __forceinline__ void epi_act(const EpiParams& e, int64_t row, int64_t
 #pragma unroll
       for (int i = 0; i < NC; ++i) acc[i] += v[i];
     }
-    row_store<E, NC>(e.out, row * e.ld_out + col, n, e.vec, acc);
+    st.template put<E, NC>(0, e.out, row, e.ld_out, col, n, e.vec, acc);
   } else if constexpr (KIND == kEpiGated) {
     if (e.gate) {
-      row_store<E, NC>(e.gate, row * e.ld_gu + col, n, e.vec, acc);
-      row_store<E, NC>(e.up, row * e.ld_gu + col, n, e.vec, acc2);
+      st.template put<E, NC>(1, e.gate, row, e.ld_gu, col, n, e.vec, acc);
+      st.template put<E, NC>(2, e.up, row, e.ld_gu, col, n, e.vec, acc2);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) v[i] = act_fwd<ACT>(acc[i]) * acc2[i];
-    row_store<E, NC>(e.out, row * e.ld_out + col, n, e.vec, v);
+    st.template put<E, NC>(0, e.out, row, e.ld_out, col, n, e.vec, v);
   } else {
     float u[NC];
     if (acc2) {  // loaded ahead: gate in v's place, then up
@@ -176,21 +185,28 @@ __device__ __forceinline__ void epi_act(const EpiParams& e, int64_t row, int64_t
       u[i] *= a;                  // h
       acc[i] *= a;                // gu
     }
-    row_store<E, NC>(e.gg, row * e.ld_g + col, n, e.vec, v);
-    row_store<E, NC>(e.gu, row * e.ld_g + col, n, e.vec, acc);
-    row_store<E, NC>(e.out, row * e.ld_out + col, n, e.vec, u);
+    st.template put<E, NC>(1, e.gg, row, e.ld_g, col, n, e.vec, v);
+    st.template put<E, NC>(2, e.gu, row, e.ld_g, col, n, e.vec, acc);
+    st.template put<E, NC>(0, e.out, row, e.ld_out, col, n, e.vec, u);
+  }
+}
+template <typename E, int KIND, int NC, typename Store>
+__device__ __forceinline__ void epi_chunk(const EpiParams& e, int64_t row, int64_t col, int n,
+                                          float* acc, const float* acc2, Store& st) {
+  switch (e.act) {  // uniform over the grid
+    case MHC_ACT_RELU: return epi_act<E, KIND, MHC_ACT_RELU, NC>(e, row, col, n, acc, acc2, st);
+    case MHC_ACT_GELU: return epi_act<E, KIND, MHC_ACT_GELU, NC>(e, row, col, n, acc, acc2, st);
+    case MHC_ACT_GELU_TANH:
+      return epi_act<E, KIND, MHC_ACT_GELU_TANH, NC>(e, row, col, n, acc, acc2, st);
+    case MHC_ACT_SILU: return epi_act<E, KIND, MHC_ACT_SILU, NC>(e, row, col, n, acc, acc2, st);
+    default: return epi_act<E, KIND, MHC_ACT_NONE, NC>(e, row, col, n, acc, acc2, st);
   }
 }
 template <typename E, int KIND, int NC>
 __device__ __forceinline__ void epi_chunk(const EpiParams& e, int64_t row, int64_t col, int n,
                                           float* acc, const float* acc2) {
-  switch (e.act) {  // uniform over the grid
-    case MHC_ACT_RELU: return epi_act<E, KIND, MHC_ACT_RELU, NC>(e, row, col, n, acc, acc2);
-    case MHC_ACT_GELU: return epi_act<E, KIND, MHC_ACT_GELU, NC>(e, row, col, n, acc, acc2);
-    case MHC_ACT_GELU_TANH: return epi_act<E, KIND, MHC_ACT_GELU_TANH, NC>(e, row, col, n, acc, acc2);
-    case MHC_ACT_SILU: return epi_act<E, KIND, MHC_ACT_SILU, NC>(e, row, col, n, acc, acc2);
-    default: return epi_act<E, KIND, MHC_ACT_NONE, NC>(e, row, col, n, acc, acc2);
-  }
+  StoreRows st;
+  epi_chunk<E, KIND, NC>(e, row, col, n, acc, acc2, st);
 }
 
 }  // namespace mhc
