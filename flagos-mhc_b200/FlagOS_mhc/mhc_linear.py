@@ -53,7 +53,9 @@ def mhc_linear(x, weight, bias=None, residual=None, activation="none", need_back
     xf, xs = _C.rows(x, D)
     wf, wstr = _C.rows(weight, D)
     rf, rs = _C.rows(residual, F) if residual is not None else (None, 0)
-    bf = bias.contiguous() if bias is not None else None
+    bf = bias
+    if bf is not None and (not bf.is_contiguous() or bf.data_ptr() & 31):
+        bf = bf.clone(memory_format=torch.contiguous_format)  # the epilogue reads it in packs
     dev = x.device
     y = torch.empty(out_shape, dtype=x.dtype, device=dev)
     z = torch.empty(out_shape, dtype=x.dtype, device=dev) if need_backward and act else None

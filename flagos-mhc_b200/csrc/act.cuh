@@ -12,6 +12,12 @@ __device__ __forceinline__ float sigmoid_fast(float z) {
   return __fdividef(1.f, 1.f + __expf(-z));
 }
 
+// The functions that vanish for z -> -inf are 0 there, and their derivatives 0 or 1 beyond either
+// end: a z kept in fp16 may have become infinite.  The factors z are clamped where the other
+// factor is exactly 0 already, so that no 0 * inf arises (NaN still passes, by the other factor).
+__device__ __forceinline__ float floor_z(float z) { return fmaxf(z, -128.f); }
+__device__ __forceinline__ float clamp_z(float z) { return fminf(fmaxf(z, -128.f), 128.f); }
+
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluK = 0.044715f;
 
@@ -39,12 +45,12 @@ __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (ACT == MHC_ACT_RELU) return z < 0.f ? 0.f : z;  // NaN passes
   if constexpr (ACT == MHC_ACT_GELU) {
     float e;
-    return z * normal_cdf(z, e);
+    return floor_z(z) * normal_cdf(z, e);
   }
   // 0.5 z (1 + tanh(u)) = z sigmoid(2u)
   if constexpr (ACT == MHC_ACT_GELU_TANH)
-    return z * sigmoid_fast(2.f * kGeluC * z * fmaf(kGeluK * z, z, 1.f));
-  if constexpr (ACT == MHC_ACT_SILU) return z * sigmoid_fast(z);
+    return floor_z(z) * sigmoid_fast(2.f * kGeluC * z * fmaf(kGeluK * z, z, 1.f));
+  if constexpr (ACT == MHC_ACT_SILU) return floor_z(z) * sigmoid_fast(z);
   return z;
 }
 
@@ -57,18 +63,18 @@ __device__ __forceinline__ void act_both(float z, float& a, float& da) {
   } else if constexpr (ACT == MHC_ACT_GELU) {
     float e;
     const float cdf = normal_cdf(z, e);
-    a = z * cdf;
-    da = fmaf(z * 0.3989422804014327f, e, cdf);
+    a = floor_z(z) * cdf;
+    da = fmaf(clamp_z(z) * 0.3989422804014327f, e, cdf);
   } else if constexpr (ACT == MHC_ACT_GELU_TANH) {
     const float s = sigmoid_fast(2.f * kGeluC * z * fmaf(kGeluK * z, z, 1.f));
-    a = z * s;
-    // beyond |z| = 12 the sigmoid is 0 or 1 in fp32; the clamp keeps 0 * inf out
+    a = floor_z(z) * s;
+    // beyond |z| = 12 the sigmoid is 0 or 1 in fp32
     const float zc = fminf(fmaxf(z, -12.f), 12.f);
     da = fmaf(zc * s * (1.f - s), 2.f * kGeluC * fmaf(3.f * kGeluK * zc, zc, 1.f), s);
   } else if constexpr (ACT == MHC_ACT_SILU) {
     const float s = sigmoid_fast(z);
-    a = z * s;
-    da = s * fmaf(z, 1.f - s, 1.f);
+    a = floor_z(z) * s;
+    da = s * fmaf(clamp_z(z), 1.f - s, 1.f);
   } else {
     a = z;
     da = 1.f;

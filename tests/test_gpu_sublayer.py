@@ -311,6 +311,28 @@ def test_activations_over_their_range():
             check(gx, da, 2 * u_of(dt) * da.abs() + act_slack(x.double().clamp(-12, 12)), name + "'")
 
 
+@pytest.mark.parametrize("T", [3, 40, 600])
+def test_activations_beyond_the_type(T):
+    """A pre-activation past fp16's range: the forward works in fp32, z is kept as infinity, and
+    the derivative there is 0 or 1."""
+    dt = torch.float16
+    x = torch.full((T, 8), 250.0, device=DEV, dtype=dt)
+    w = torch.zeros(16, 8, device=DEV, dtype=dt)
+    w[0], w[1] = 250.0, -250.0            # z = 5e5, -5e5
+    gy = torch.ones(T, 16, device=DEV, dtype=dt)
+    for name in ("relu", "gelu", "gelu_tanh", "silu"):
+        o = M.mhc_linear(x, w, activation=name, need_backward=True)
+        assert torch.isinf(o["z"][:, :2]).all() and (o["y"][:, 1:] == 0).all()
+        gx, gw, gb = M.mhc_linear_backward(x, w, o["z"], gy, activation=name)
+        assert torch.isfinite(gx).all() and (gx[:, 0] == 250.0).all(), name
+        assert gb[0] == T and gb[1] == 0
+    up = torch.ones_like(w)
+    f = M.mhc_gated_ffn(x / 250, w * 400, up / 8, w.t().contiguous() * 0 + 1, need_backward=True)
+    g = M.mhc_gated_ffn_backward(x / 250, w * 0, up / 8, w.t().contiguous() * 0 + 1,
+                                 torch.full_like(f["gate"], float("-inf")), f["up"], x / 250)
+    assert all(torch.isfinite(t).all() for t in g)
+
+
 def test_rows_keep_to_themselves():
     """NaN and infinity in one token reach that token's outputs only."""
     for T in (6, 200):
@@ -485,6 +507,42 @@ def test_graph_replay_matches_eager(T, D, F):
             assert torch.equal(a, b), (rep, i)
     from FlagOS_mhc import _C
     assert _C.lib().mhc_device_status() == 0
+
+
+@pytest.mark.parametrize("T", [5, 300])
+def test_captured_training_step(T):
+    """Forward and backward through the autograd wrappers, captured once and replayed on new
+    inputs, against the eager step (made after the graph's own leaves are done with)."""
+    D, F = 136, 264
+
+    def leaves(d):
+        return {k: d[k].clone().requires_grad_() for k in ("x", "lw", "lb", "wg", "wu", "wd", "w", "b")}
+
+    def step(q, gy):
+        h = M.mhc_gated_ffn_fn(M.mhc_layer_norm_fn(q["x"], q["lw"], q["lb"]), q["wg"], q["wu"], q["wd"])
+        y = M.mhc_linear_fn(h, q["w"], q["b"], residual=q["x"], activation="gelu")
+        return [y.detach(), *torch.autograd.grad(y, list(q.values()), gy)]
+
+    d = sub_inputs(T, D, F, torch.bfloat16, seed=3)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        q = leaves(d)
+        step(q, d["gy"])                   # warm-up on the capturing stream
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        outs = step(q, d["gy"])
+    for seed in (21, 22):
+        new = sub_inputs(T, D, F, torch.bfloat16, seed=seed)
+        with torch.no_grad():
+            for k in q:
+                q[k].copy_(new[k])
+        d["gy"].copy_(new["gy"])
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, (a, b) in enumerate(zip(outs, step(leaves(new), new["gy"]))):
+            assert torch.equal(a, b), (seed, i)
 
 
 @pytest.mark.parametrize("T,D,F", SUB)
