@@ -473,7 +473,8 @@ static int64_t part_ld(const Gemm& g) { return cdiv(g.N, 32) * 32; }
 
 // The cut whose estimated time (us) is least.  Measured: 7 us to start and end a launch; 0.36 us
 // to a K block of a 256-row tile and 0.73 us of a 512-row one in a short run, 0.50 and 0.86 us
-// under the power cap (the 512-row tile reads B half as often for its work).  The 512-row tile's
+// under the power cap (the 512-row tile reads B half as often for its work), and 0.28 and 0.56 us
+// with few clusters at work; the constants lie between.  The 512-row tile's
 // epilogue, with no accumulators left for the next tile, stands alone: 2 us, 3 us with a gate,
 // 20 us with the gate's backward.  A cut in K writes and reads fp32 partials (at 4 TB/s) and
 // takes another launch (3 us).
@@ -488,12 +489,13 @@ static GemmPlan gemm_plan(const Gemm& g) {
   for (int mt = 1; mt <= 2; ++mt) {
     if (mt == 2 && g.M <= 256) break;
     const int64_t tiles = cdiv(g.M, 256 * mt) * tn;
-    const double per_k = mt == 1 ? 0.40 : 0.75;
     const double tail = mt == 1 ? 1.0 : g.kind == kEpiLinear ? 2.0 : dual ? 3.0 : 20.0;
     for (int sp = 1; sp <= 16; ++sp) {
       // (beyond eight waves a cut gains nothing)
       if (sp > 1 && (nk < 4 * sp || plane * sp * 4 > 1e9 || tiles * (sp - 1) > 8 * clusters)) break;
       const double waves = (double)cdiv(tiles * sp, clusters);
+      const double busy = std::min(1.0, (double)(tiles * sp) / (double)clusters);
+      const double per_k = mt == 1 ? 0.28 + 0.12 * busy : 0.56 + 0.19 * busy;
       double us = 7.0 + waves * ((double)cdiv(nk, sp) * per_k + tail);
       if (sp > 1) us += 3.0 + plane * sp * 8 / 4e6;
       if (us < best_us) best_us = us, best = {mt, sp, 0};

@@ -300,7 +300,8 @@ static int few_launch(const Gemm& g, int splits, cudaStream_t s) {
 
 // The tile and the cut in K whose estimated time (us) is least; 0 if this form does not take the
 // product.  Measured: 4 us to start and end a launch; to a K block 0.17 us, or its bytes at 130
-// GB/s an SM and 14 TB/s in all; at a tile's end 0.6 us and 0.016 us a token; the weights at 6.4 TB/s after 6 us.
+// GB/s an SM and 14 TB/s in all; at a tile's end 0.6 us and 0.016 us a token, and with a cut in K
+// 0.8 us and 0.012 us a token more; the weights at 6.4 TB/s after 6 us.
 // (Clusters of 8 CTAs of this size leave SMs empty: 1024 -> 2048 features, T=128: 22 us against
 // 9.6 with 2.)
 double few_estimate(const Gemm& g, int* nt_best, int* splits) {
@@ -318,7 +319,7 @@ double few_estimate(const Gemm& g, int* nt_best, int* splits) {
       const double waves = (double)cdiv(tiles * sp, sm_count());
       const double active = (double)std::min<int64_t>(tiles * sp, sm_count());
       const double per_k = std::max(0.17 * W, std::max(bytes / 130e3, bytes * active / 14e6));
-      double us = 4.0 + (sp > 1 ? 0.8 : 0.0) +
+      double us = 4.0 + (sp > 1 ? 0.8 + 0.012 * W * nt : 0.0) +
                   waves * ((double)cdiv(nk, sp) * per_k + 0.6 + 0.016 * W * nt);
       us = std::max(us, hbm);
       if (us < best) best = us, *nt_best = nt, *splits = sp;
