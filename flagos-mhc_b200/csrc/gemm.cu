@@ -638,35 +638,67 @@ int gemm_run(const Gemm& g0, void* ws, cudaStream_t s) {
 int gemm_device_error() { return read_and_clear_tu_error(); }
 
 // ---------------------------------------------------------------- packed copies
-// Rows of an operand that TMA cannot address (base or row stride off 16 bytes), copied to
-// rows that start on 16-byte boundaries.
-template <int V>  // bytes per access
+// Rows of 2-byte elements, copied between matrices whose rows start anywhere.  A thread writes
+// one 16-byte chunk of a row, aligned in the destination; its source, shifted against that, comes
+// from the two aligned 16-byte words that hold it (a warp's threads share them in L1).  Bound by
+// HBM; with an element to a thread the 6704 x 11861 weight took 300 us of a gated block's 430.
+// `begin`, `end`: the source matrix, past which no word is read.
+template <typename I>  // of the chunks' count
 __global__ void __launch_bounds__(256)
-    pack_rows_kernel(const char* __restrict__ src, int64_t ls, int64_t rows, int64_t row_bytes,
-                     char* __restrict__ dst, int64_t ld) {
+    pack_rows_kernel(const char* __restrict__ src, int64_t ls, int64_t rows, int64_t cols,
+                     char* __restrict__ dst, int64_t ld, const char* begin, const char* end) {
   pdl_enter();
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < row_bytes;
-         i += (int64_t)gridDim.x * 256 * V) {
-      if constexpr (V == 4)
-        *(uint32_t*)(dst + r * ld + i) = __ldg((const uint32_t*)(src + r * ls + i));
-      else
-        *(uint16_t*)(dst + r * ld + i) = __ldg((const uint16_t*)(src + r * ls + i));
+  const I per = (I)((cols + 7) / 8 + 1), total = (I)rows * per;  // a row may touch one chunk more
+  for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < total; i += (I)gridDim.x * 256) {
+    const I r = i / per;
+    const char* sp = src + (int64_t)r * ls;
+    char* dp = dst + (int64_t)r * ld;
+    const int64_t e0 = (int64_t)(i - r * per) * 8 - (int64_t)((reinterpret_cast<uintptr_t>(dp) & 15) >> 1);
+    if (e0 >= cols) continue;
+    if (e0 >= 0 && e0 + 8 <= cols) {
+      const char* sa = sp + e0 * 2;
+      const int sh = (int)((reinterpret_cast<uintptr_t>(sa) & 15) >> 1);  // elements
+      const char* a0 = sa - 2 * sh;
+      uint32_t w[8];
+      if (sh == 0 || (a0 >= begin && a0 + 32 <= end)) {
+        const uint4 lo = *reinterpret_cast<const uint4*>(a0);
+        const uint4 hi = sh ? *reinterpret_cast<const uint4*>(a0 + 16) : make_uint4(0, 0, 0, 0);
+        w[0] = lo.x; w[1] = lo.y; w[2] = lo.z; w[3] = lo.w;
+        w[4] = hi.x; w[5] = hi.y; w[6] = hi.z; w[7] = hi.w;
+        if (sh & 4) {
+#pragma unroll
+          for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+        }
+        if (sh & 2) {
+#pragma unroll
+          for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+        }
+        if (sh & 1) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+        }
+      } else {
+        const uint16_t* se = reinterpret_cast<const uint16_t*>(sa);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = se[2 * k] | (uint32_t)se[2 * k + 1] << 16;
+      }
+      *reinterpret_cast<uint4*>(dp + e0 * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      const int64_t e1 = e0 + 8 < cols ? e0 + 8 : cols;
+      for (int64_t e = e0 > 0 ? e0 : 0; e < e1; ++e)
+        *reinterpret_cast<uint16_t*>(dp + 2 * e) = *reinterpret_cast<const uint16_t*>(sp + 2 * e);
     }
+  }
 }
 
 int pack_rows(const void* src, int64_t ls, int64_t rows, int64_t cols, void* dst, int64_t ld,
               cudaStream_t s) {
-  const bool four = ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 3) == 0 &&
-                    ls % 2 == 0 && ld % 2 == 0 && cols % 2 == 0;
-  const dim3 grid((unsigned)std::min<int64_t>(cdiv(cols * 2, 256 * (four ? 4 : 2)), 64),
-                  (unsigned)std::min<int64_t>(rows, 16384));
-  if (four)
-    launch(pack_rows_kernel<4>, grid, 256, 0, s, (const char*)src, ls * 2, rows, cols * 2,
-           (char*)dst, ld * 2);
-  else
-    launch(pack_rows_kernel<2>, grid, 256, 0, s, (const char*)src, ls * 2, rows, cols * 2,
-           (char*)dst, ld * 2);
+  const char* begin = (const char*)src;
+  const char* end = begin + ((rows - 1) * ls + cols) * 2;
+  const int64_t total = rows * ((cols + 7) / 8 + 1);
+  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(total, 256), 32 * sm_count());
+  launch(total < INT32_MAX / 2 ? pack_rows_kernel<uint32_t> : pack_rows_kernel<uint64_t>, grid, 256, 0, s,
+         begin, ls * 2, rows, cols, (char*)dst, ld * 2, begin, end);
   MHC_LAUNCH_CHECK();
   return MHC_OK;
 }
