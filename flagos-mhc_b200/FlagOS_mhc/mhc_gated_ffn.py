@@ -50,7 +50,9 @@ def mhc_gated_ffn(x, w_gate, w_up, w_down, activation="silu", need_backward=Fals
     gate = up = None
     ld = (F + 15) // 16 * 16  # rows start on 32-byte boundaries
     if need_backward:
-        gate, up = torch.empty(2, T, ld, dtype=x.dtype, device=dev)[:, :, :F].unbind(0)
+        gate, up = (torch.empty(T, ld, dtype=x.dtype, device=dev) for _ in range(2))
+        if ld != F:
+            gate, up = gate[:, :F], up[:, :F]
     L = _C.lib()
     with _C.device_guard(dev):
         nbytes = L.mhc_gated_ffn_fwd_workspace_bytes(
