@@ -1,5 +1,5 @@
 """The sublayer operators (layer norm, linear layer, gated feed-forward block) in float64,
-from their formulas: the checker of the CUDA kernels.  Any device."""
+from their formulas: what the CUDA kernels are tested against.  Any device."""
 import math
 
 import torch
