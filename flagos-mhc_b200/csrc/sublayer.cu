@@ -90,8 +90,14 @@ __global__ void __launch_bounds__(256)
   const int64_t f = (int64_t)blockIdx.x * 32 + lane;
   Kahan k;
   if (f < F) {
-#pragma unroll 8
-    for (int i = ranges * seg / 8; i < ranges * (seg + 1) / 8; ++i) k.add(part[(int64_t)i * F + f]);
+const int i0 = ranges * seg / 8, i1 = ranges * (seg + 1) / 8;
+    for (int i = i0; i < i1; i += 8) {
+      float v[8];  // loads in flight together, past the range 0
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + j < i1 ? part[(int64_t)(i + j) * F + f] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k.add(v[j]);
+    }
   }
   sum[seg][lane] = k.s;
   __syncthreads();
