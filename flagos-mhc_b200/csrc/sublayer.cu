@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256)
   const int64_t f = (int64_t)blockIdx.x * 32 + lane;
   Kahan k;
   if (f < F) {
-const int i0 = ranges * seg / 8, i1 = ranges * (seg + 1) / 8;
+    const int i0 = ranges * seg / 8, i1 = ranges * (seg + 1) / 8;
     for (int i = i0; i < i1; i += 8) {
       float v[8];  // loads in flight together, past the range 0
 #pragma unroll
