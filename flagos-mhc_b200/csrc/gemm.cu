@@ -1,12 +1,16 @@
 // gemm.cu -- the matrix product of gemm.cuh on tcgen05, with the operators' epilogues.
 //
-// A cluster of two CTAs owns a 256 x 256 tile (cta_group::2): each CTA keeps 128 rows of A
-// and half of the tile's B rows per 64-deep K block in shared memory, and 128 x 256 fp32
-// accumulators in TMEM, of which there are two sets: the epilogue of one tile runs beside
-// the products of the next.  Warp 0 loads (TMA, 6 stages of 32 KB), one thread of the
-// leader CTA issues the MMAs of both, eight warps run the epilogue.  For the gated kinds of
-// product the leader's B rows are the gate projection's and its peer's the up projection's,
-// so both values of one hidden element meet in one thread.
+// A cluster of two CTAs owns a tile of 512 or 256 rows and 256 columns (cta_group::2): of a
+// 64-deep K block each CTA keeps 128 or 256 rows of A and half of the tile's B rows in shared
+// memory (4 stages of 48 KB, or 6 of 32 KB).  Warp 0 loads (TMA), one thread of the leader CTA
+// issues the MMAs of both, eight warps run the epilogue.  Bound by the tensor pipe where K is
+// long, and before it by what L2 can feed the SMs: 256-row tiles ran at 1150-1200 TFLOP/s
+// (8192^3; 1460 with the loads left out), 512-row tiles, which read B half as often, at
+// 1400-1580.  Their two accumulators of 128 x 256 fp32 fill TMEM, so a tile's epilogue runs
+// alone; with 256 rows there are two sets, and it runs beside the products of the next tile,
+// which the long epilogue of the gate's backward needs.  For the gated kind of product the
+// leader's B rows are the gate projection's and its peer's the up projection's, so both values
+// of one hidden element meet in one thread.
 //
 // Either operand may be K-major or MN-major (the transposed products of the backward): only
 // the TMA box and the shared-memory descriptor differ.  Rows and columns past the edges are
