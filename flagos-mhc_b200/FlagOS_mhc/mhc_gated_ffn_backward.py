@@ -40,7 +40,8 @@ def mhc_gated_ffn_backward(x, w_gate, w_up, w_down, gate, up, grad_y, activation
     L = _C.lib()
     with _C.device_guard(x.device):
         nbytes = L.mhc_gated_ffn_bwd_workspace_bytes(
-            T, D, F, code, _C.unaligned((xf, xs), (wg, wgs), (wu, wus), (wd, wds), (gf, gs), (wg, D), (wd, F)))
+            T, D, F, code, _C.unaligned((xf, xs), (wg, wgs), (wu, wus), (wd, wds), (gf, gs),
+                                        *zip(outs, (D, D, D, F))))
         ws, wp = _C.workspace(nbytes, x.device)
         st = L.mhc_gated_ffn_bwd(_C.addr(xf), xs, _C.addr(wg), wgs, _C.addr(wu), wus, _C.addr(wd), wds,
                                  _C.addr(ga), _C.addr(ua), gas, _C.addr(gf), gs, T, D, F, code, act,

@@ -323,8 +323,9 @@ int mhc_pre_fwd_noalloc(const void* x, const float* phi, const float* alpha,
  * consecutive rows, the elements of a row are contiguous.  A matrix is
  * "aligned" if its base is a multiple of 16 bytes and its row stride a multiple
  * of 16 bytes; others are accepted and cost a packed copy in the workspace.
- * The workspace queries take `unaligned`: 0 if every matrix (x, weights,
- * residual, grad_y, y and the gradients) is aligned, 1 otherwise.  T = 0 is valid: parameter gradients are
+ * The workspace queries take `unaligned`: 0 if every matrix of the call (x,
+ * weights, residual, grad_y, y and the gradients) is aligned, 1 otherwise; a
+ * matrix that is NULL does not count.  T = 0 is valid: parameter gradients are
  * then zero.  MHC_F32 is taken by the layer norm only (the matrix products
  * return MHC_ERR_UNSUPPORTED_DTYPE).  Sums are held in fp32 and added in a
  * fixed order; each output is rounded once. */

@@ -1,0 +1,48 @@
+"""Calls of the sublayer operators that the documentation allows, apart from sizes and values:
+outputs that are not wanted, rows inside wider buffers."""
+import itertools
+
+import pytest
+import torch
+
+import FlagOS_mhc as M
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DT = torch.bfloat16
+
+
+def rnd(*shape, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randn(*shape, generator=g, device=DEV).to(DT)
+
+
+def padded(t):
+    """The same rows, 16-byte aligned inside a wider buffer of NaN."""
+    n = t.shape[1]
+    buf = torch.full((t.shape[0], (n + 7) // 8 * 8 + 8), float("nan"), device=DEV, dtype=DT)
+    buf[:, :n] = t
+    return buf[:, :n]
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("T,D,F", [(6, 1001, 64), (200, 1001, 64), (200, 129, 255), (600, 64, 71)])
+def test_any_subset_of_gradients_of_padded_rows(T, D, F, act):
+    x, w, wu = rnd(T, D, seed=1), rnd(F, D, seed=2) / 8, rnd(F, D, seed=3) / 8
+    wd, gy, gf = rnd(D, F, seed=4) / 8, rnd(T, D, seed=5), rnd(T, F, seed=6)
+    z = M.mhc_linear(x, w, activation=act, need_backward=True)["z"]
+    full = M.mhc_linear_backward(x, w, z, gf, activation=act)
+    zp = padded(z) if z is not None else None
+    for need in itertools.product((False, True), repeat=3):
+        got = M.mhc_linear_backward(padded(x), padded(w), zp, padded(gf), activation=act,
+                                    need_x_grad=need[0], need_weight_grad=need[1],
+                                    need_bias_grad=need[2])
+        for n, p, q in zip(need, got, full):
+            assert torch.equal(p, q) if n else p is None, need
+    o = M.mhc_gated_ffn(x, w, wu, wd, activation=act, need_backward=True)
+    full = M.mhc_gated_ffn_backward(x, w, wu, wd, o["gate"], o["up"], gy, activation=act)
+    for need in itertools.product((False, True), repeat=4):
+        got = M.mhc_gated_ffn_backward(padded(x), padded(w), padded(wu), padded(wd), o["gate"],
+                                       o["up"], padded(gy), activation=act, need_grads=need)
+        for n, p, q in zip(need, got, full):
+            assert torch.equal(p, q) if n else p is None, need
