@@ -25,6 +25,9 @@ def mhc_gated_ffn_backward(x, w_gate, w_up, w_down, gate, up, grad_y, activation
     _C.require_cuda(x, w_gate, w_up, w_down, gate, up, grad_y)
     code = _matrix_dtype(x)
     _C.require_same("mhc_gated_ffn_backward", x, w_gate, w_up, w_down, gate, up, grad_y)
+    need_grads = tuple(need_grads)
+    if not any(need_grads):
+        return (None,) * 4
     xf, xs = _C.rows(x, D)
     wg, wgs = _C.rows(w_gate, D)
     wu, wus = _C.rows(w_up, D)

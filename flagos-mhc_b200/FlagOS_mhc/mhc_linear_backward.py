@@ -29,6 +29,8 @@ def mhc_linear_backward(x, weight, z, grad_y, activation="none", need_x_grad=Tru
     _C.require_cuda(x, weight, z, grad_y)
     code = _matrix_dtype(x)
     _C.require_same("mhc_linear_backward", x, weight, z, grad_y)
+    if not (need_x_grad or need_weight_grad or need_bias_grad):
+        return (None,) * 3
     xf, xs = _C.rows(x, D)
     wf, wstr = _C.rows(weight, D)
     gf, gs = _C.rows(grad_y, F)

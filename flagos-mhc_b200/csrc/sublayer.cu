@@ -318,6 +318,7 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
   const cudaStream_t s = (cudaStream_t)stream;
   if (T > 0 && (!x || !weight || !grad_y || (act != MHC_ACT_NONE && !z)))
     return MHC_ERR_INVALID_ARGUMENT;
+  if (!grad_x && !grad_weight && !grad_bias) return MHC_OK;
   Operand ox{x, x_stride, false}, ow{weight, weight_stride, false};
   const bool gy_packed = act == MHC_ACT_NONE && !operand_aligned({grad_y, grad_y_stride, false});
   if (T > 0 && !ws_ok(workspace, workspace_bytes,
@@ -458,6 +459,7 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
   const cudaStream_t s = (cudaStream_t)stream;
   if (T > 0 && (!x || !w_gate || !w_up || !w_down || !gate || !up || !grad_y))
     return MHC_ERR_INVALID_ARGUMENT;
+  if (!grad_x && !grad_w_gate && !grad_w_up && !grad_w_down) return MHC_OK;
   Operand ox{x, x_stride, false}, oy{grad_y, grad_y_stride, true},
       og{w_gate, w_gate_stride, false}, ou{w_up, w_up_stride, false},
       od{w_down, w_down_stride, false};

@@ -46,3 +46,24 @@ def test_any_subset_of_gradients_of_padded_rows(T, D, F, act):
                                        o["up"], padded(gy), activation=act, need_grads=need)
         for n, p, q in zip(need, got, full):
             assert torch.equal(p, q) if n else p is None, need
+
+
+def launches():
+    from FlagOS_mhc import _C
+    return _C.lib().mhc_kernel_launches()
+
+
+def test_a_backward_without_outputs_launches_nothing():
+    T, D, F = 40, 136, 72
+    x, w, gy, gf = rnd(T, D, seed=1), rnd(F, D, seed=2), rnd(T, D, seed=3), rnd(T, F, seed=4)
+    wd = rnd(D, F, seed=5)
+    n = launches()
+    assert M.mhc_linear_backward(x, w, gf, gf, activation="silu", need_x_grad=False,
+                                 need_weight_grad=False, need_bias_grad=False) == (None,) * 3
+    assert M.mhc_gated_ffn_backward(x, w, w, wd, gf, gf, gy, need_grads=(False,) * 4) == (None,) * 4
+    assert launches() == n
+    some = M.mhc_gated_ffn_backward(x, w, w, wd, gf, gf, gy, need_grads=(i == 2 for i in range(4)))
+    assert [t is None for t in some] == [True, True, False, True]
+    with pytest.raises(AssertionError):     # the arguments are checked all the same
+        M.mhc_linear_backward(x, w, gf, gy, activation="silu", need_x_grad=False,
+                              need_weight_grad=False, need_bias_grad=False)

@@ -66,3 +66,20 @@ def test_gated_ffn_takes_the_queried_workspace(T, D, F, pad):
         n = L.mhc_gated_ffn_bwd_workspace_bytes(T, D, F, 2, int(un))
         passes(L.mhc_gated_ffn_bwd(P, d, P, d, P, d, P, f, P, P, f, P, d, T, D, F, 2, 4, gx, gg, gu,
                                    gd, WS, n, None))
+
+
+def test_a_backward_without_outputs_has_nothing_to_do():
+    """No device, no workspace: the calls return before either is asked for."""
+    L = _C.lib()
+    for act, z in ((0, None), (4, P)):
+        for T in (0, 4, 200):
+            assert L.mhc_linear_bwd(P, 16, P, 16, z, 8, P, 8, T, 16, 8, 2, act, None, None, None, None,
+                                    0, None) == _C.MHC_OK
+    for T in (0, 4, 200):
+        assert L.mhc_gated_ffn_bwd(P, 16, P, 16, P, 16, P, 8, P, P, 8, P, 16, T, 16, 8, 2, 4, None,
+                                   None, None, None, None, 0, None) == _C.MHC_OK
+    # the arguments are checked all the same
+    assert L.mhc_linear_bwd(P, 16, P, 16, None, 8, P, 8, 4, 16, 8, 2, 4, None, None, None, None, 0,
+                            None) == _C.MHC_ERR_INVALID_ARGUMENT
+    assert L.mhc_gated_ffn_bwd(P, 16, P, 16, P, 16, P, 8, P, None, 8, P, 16, 4, 16, 8, 2, 4, None, None,
+                               None, None, None, 0, None) == _C.MHC_ERR_INVALID_ARGUMENT
