@@ -110,6 +110,12 @@ def mhc_pre_clamp_sinkhorn_fn(x, phi, alpha, base, norm_eps=1e-6, hc_eps=1e-6, c
                                        clamp_max, iter_times, materialize_x_scaled, premix)
 
 
+def _graph_wanted(*tensors):
+    """Whether a call made now is differentiated later.  Asked before Function.apply, which turns
+    the grad mode off around its forward."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class MhcLayerNormFn(torch.autograd.Function):
     """Layer norm; saves (x, weight, mean, rstd)."""
 
@@ -137,13 +143,14 @@ def mhc_layer_norm_fn(x, weight=None, bias=None, eps=1e-5):
 
 
 class MhcLinearFn(torch.autograd.Function):
-    """Linear layer; saves (x, weight, z)."""
+    """Linear layer; saves (x, weight, z), nothing with ``keep`` false."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
+    def forward(ctx, x, weight, bias, residual, activation, keep=True):
         out = mhc_linear(x, weight, bias=bias, residual=residual, activation=activation,
-                         need_backward=True)
-        ctx.save_for_backward(x, weight, out["z"])
+                         need_backward=keep)
+        if keep:
+            ctx.save_for_backward(x, weight, out["z"])
         ctx.activation = activation
         return out["y"]
 
@@ -154,21 +161,24 @@ class MhcLinearFn(torch.autograd.Function):
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
         gx, gw, gb = mhc_linear_backward(x, weight, z, grad_y, activation=ctx.activation,
                                          need_x_grad=nx, need_weight_grad=nw, need_bias_grad=nb)
-        return gx, gw, gb, grad_y if nr else None, None
+        return gx, gw, gb, grad_y if nr else None, None, None
 
 
 def mhc_linear_fn(x, weight, bias=None, residual=None, activation="none"):
-    """Autograd-aware mhc_linear. Returns y."""
-    return MhcLinearFn.apply(x, weight, bias, residual, activation)
+    """Autograd-aware mhc_linear. Returns y.  z is written only if a gradient is wanted."""
+    return MhcLinearFn.apply(x, weight, bias, residual, activation,
+                             _graph_wanted(x, weight, bias, residual))
 
 
 class MhcGatedFfnFn(torch.autograd.Function):
-    """Gated feed-forward block; saves (x, w_gate, w_up, w_down, gate, up)."""
+    """Gated feed-forward block; saves (x, w_gate, w_up, w_down, gate, up), nothing with ``keep``
+    false."""
 
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, activation):
-        out = mhc_gated_ffn(x, w_gate, w_up, w_down, activation=activation, need_backward=True)
-        ctx.save_for_backward(x, w_gate, w_up, w_down, out["gate"], out["up"])
+    def forward(ctx, x, w_gate, w_up, w_down, activation, keep=True):
+        out = mhc_gated_ffn(x, w_gate, w_up, w_down, activation=activation, need_backward=keep)
+        if keep:
+            ctx.save_for_backward(x, w_gate, w_up, w_down, out["gate"], out["up"])
         ctx.activation = activation
         return out["y"]
 
@@ -176,9 +186,11 @@ class MhcGatedFfnFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_y):
         return mhc_gated_ffn_backward(*ctx.saved_tensors, grad_y, activation=ctx.activation,
-                                      need_grads=ctx.needs_input_grad[:4]) + (None,)
+                                      need_grads=ctx.needs_input_grad[:4]) + (None, None)
 
 
 def mhc_gated_ffn_fn(x, w_gate, w_up, w_down, activation="silu"):
-    """Autograd-aware mhc_gated_ffn. Returns y."""
-    return MhcGatedFfnFn.apply(x, w_gate, w_up, w_down, activation)
+    """Autograd-aware mhc_gated_ffn. Returns y.  gate and up are written only if a gradient is
+    wanted."""
+    return MhcGatedFfnFn.apply(x, w_gate, w_up, w_down, activation,
+                               _graph_wanted(x, w_gate, w_up, w_down))

@@ -67,3 +67,21 @@ def test_a_backward_without_outputs_launches_nothing():
     with pytest.raises(AssertionError):     # the arguments are checked all the same
         M.mhc_linear_backward(x, w, gf, gy, activation="silu", need_x_grad=False,
                               need_weight_grad=False, need_bias_grad=False)
+
+
+def test_wrappers_without_grad_mode_allocate_the_output_alone():
+    T, D, F = 2048, 256, 4096
+    x, w, wu = (t.requires_grad_() for t in (rnd(T, D, seed=1), rnd(F, D, seed=2), rnd(F, D, seed=3)))
+    wd = (rnd(D, F, seed=4) / 64).requires_grad_()
+    for call in (lambda: M.mhc_linear_fn(x, w, activation="silu"),
+                 lambda: M.mhc_gated_ffn_fn(x, w, wu, wd)):
+        want = call()
+        torch.cuda.synchronize()
+        base = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        with torch.no_grad():
+            got = call()
+        peak = torch.cuda.max_memory_allocated() - base
+        assert torch.equal(got, want) and not got.requires_grad
+        # the linear layer's y; the gated block's y and, in its workspace, h
+        assert peak < 1.5 * T * F * 2, peak
