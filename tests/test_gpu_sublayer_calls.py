@@ -69,19 +69,26 @@ def test_a_backward_without_outputs_launches_nothing():
                               need_weight_grad=False, need_bias_grad=False)
 
 
-def test_wrappers_without_grad_mode_allocate_the_output_alone():
+def peak_of(call):
+    """Bytes that a call takes at most, its result among them."""
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = call()
+    return out, torch.cuda.max_memory_allocated() - base
+
+
+def test_wrappers_without_grad_mode_take_what_the_operator_takes():
     T, D, F = 2048, 256, 4096
     x, w, wu = (t.requires_grad_() for t in (rnd(T, D, seed=1), rnd(F, D, seed=2), rnd(F, D, seed=3)))
     wd = (rnd(D, F, seed=4) / 64).requires_grad_()
-    for call in (lambda: M.mhc_linear_fn(x, w, activation="silu"),
-                 lambda: M.mhc_gated_ffn_fn(x, w, wu, wd)):
-        want = call()
-        torch.cuda.synchronize()
-        base = torch.cuda.memory_allocated()
-        torch.cuda.reset_peak_memory_stats()
+    for fn, op in ((lambda: M.mhc_linear_fn(x, w, activation="silu"),
+                    lambda: M.mhc_linear(x, w, activation="silu")["y"]),
+                   (lambda: M.mhc_gated_ffn_fn(x, w, wu, wd),
+                    lambda: M.mhc_gated_ffn(x, w, wu, wd)["y"])):
         with torch.no_grad():
-            got = call()
-        peak = torch.cuda.max_memory_allocated() - base
-        assert torch.equal(got, want) and not got.requires_grad
-        # the linear layer's y; the gated block's y and, in its workspace, h
-        assert peak < 1.5 * T * F * 2, peak
+            want, least = peak_of(op)
+            got, peak = peak_of(fn)
+        assert torch.equal(got, want) and not got.requires_grad and peak == least
+        kept, more = peak_of(fn)
+        assert torch.equal(kept, want) and kept.requires_grad and more >= least + T * F * 2
