@@ -31,6 +31,7 @@ int post_mix_run(const void* x, const float* h_res, const void* h_out, const flo
                  void* out, int64_t T, int64_t D, int32_t dtype, const float* phi_next,
                  float* premix, int32_t layers, void* ws, cudaStream_t s);
 int tc_host_device_error();
+int bind_context(int dev);
 int gemm_device_error();
 int gemm_few_device_error();
 int layer_norm_device_error();
@@ -78,9 +79,8 @@ int check_device() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return MHC_ERR_CUDA;
   if (dev < 0 || dev >= 64) return MHC_ERR_DEVICE;
-  // A thread that has made no runtime call yet (autograd's, for one) has no current context,
-  // and the tensor-map encoder, a driver call, fails there: this binds the device's.
-  if (cudaSetDevice(dev) != cudaSuccess) return MHC_ERR_CUDA;
+  const int st = bind_context(dev);
+  if (st != MHC_OK) return st;
   if (g_arch_ok[dev] == 0) {
     int major = 0, minor = 0;
     if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||

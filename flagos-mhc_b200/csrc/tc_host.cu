@@ -25,6 +25,26 @@ static EncodeTiledFn encoder() {
   return fn;
 }
 
+// The context that a call runs in is the one that is current: a host may have made it itself,
+// with its pointers and streams.  Only a thread that has none yet (autograd's, for one, before its
+// first runtime call) is given the device's own, since the tensor-map encoder, a driver call, fails
+// without.
+int bind_context(int dev) {
+  typedef CUresult (*CurrentFn)(CUcontext*);
+  static CurrentFn current = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      current = reinterpret_cast<CurrentFn>(p);
+  });
+  CUcontext ctx = nullptr;
+  if (current && current(&ctx) == CUDA_SUCCESS && ctx) return MHC_OK;
+  return cudaSetDevice(dev) == cudaSuccess ? MHC_OK : MHC_ERR_CUDA;
+}
+
 int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem,
                  uint64_t cols, uint64_t rows, uint64_t row_stride_bytes, uint32_t box_cols,
                  uint32_t box_rows, CUtensorMapSwizzle swz) {

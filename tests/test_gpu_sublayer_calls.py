@@ -92,3 +92,31 @@ def test_wrappers_without_grad_mode_take_what_the_operator_takes():
         assert torch.equal(got, want) and not got.requires_grad and peak == least
         kept, more = peak_of(fn)
         assert torch.equal(kept, want) and kept.requires_grad and more >= least + T * F * 2
+
+
+def test_a_hosts_own_context_stays_current():
+    """A host that made its context with the driver API finds it current after a call; the pointers
+    and streams that it hands over belong to it.  The call is one without device work."""
+    import ctypes
+    import threading
+    from FlagOS_mhc import _C
+    cu = ctypes.CDLL("libcuda.so.1")
+    torch.zeros(1, device=DEV)              # the driver is initialised
+    seen = {}
+
+    def host():
+        mine, now = ctypes.c_void_p(), ctypes.c_void_p()
+        seen["made"] = cu.cuCtxCreate_v2(ctypes.byref(mine), 0, torch.cuda.current_device())
+        if seen["made"]:
+            return
+        p = ctypes.c_void_p(1 << 20)
+        seen["status"] = _C.lib().mhc_gated_ffn_bwd(p, 16, p, 16, p, 16, p, 8, p, p, 8, p, 16, 0, 16, 8,
+                                                    2, 4, p, None, None, None, None, 0, None)
+        cu.cuCtxGetCurrent(ctypes.byref(now))
+        seen["kept"] = now.value == mine.value
+        cu.cuCtxDestroy_v2(mine)
+
+    th = threading.Thread(target=host)
+    th.start()
+    th.join()
+    assert seen == {"made": 0, "status": 0, "kept": True}
