@@ -87,6 +87,7 @@ _SIGS = {
     "mhc_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _i32]),
     "mhc_layer_norm_bwd": (ctypes.c_int, [_vp, _i64, _fp, _fp, _fp, _vp, _i64, _i64, _i64, _i32,
                                           _vp, _fp, _fp, _vp, _sz, _vp]),
+    "mhc_sublayer_plan": (ctypes.c_int, [_i32, _i64, _i64, _i64] + [ctypes.POINTER(_i32)] * 3),
     "mhc_linear_fwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
     "mhc_linear_fwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
                                       _i32, _i32, _vp, _vp, _vp, _sz, _vp]),

@@ -467,11 +467,6 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// How a product is cut: mt accumulators of 256 rows to a tile, or 0: the form of gemm_few.cu
-// with nt tokens to a tile; `splits` ranges of K.
-struct GemmPlan {
-  int mt, splits, nt;
-};
 static int64_t k_blocks(const Gemm& g) { return cdiv(g.K, gk::BK) + cdiv(g.K3, gk::BK); }
 static int64_t part_ld(const Gemm& g) { return cdiv(g.N, 32) * 32; }
 
@@ -482,7 +477,7 @@ static int64_t part_ld(const Gemm& g) { return cdiv(g.N, 32) * 32; }
 // epilogue, with no accumulators left for the next tile, stands alone: 2 us, 3 us with a gate,
 // 20 us with the gate's backward.  A cut in K writes and reads fp32 partials (at 4 TB/s) and
 // takes another launch (3 us).
-static GemmPlan gemm_plan(const Gemm& g) {
+GemmPlan gemm_plan(const Gemm& g) {
   const bool dual = g.kind == kEpiGated;
   const int64_t nk = k_blocks(g), clusters = sm_count() / 2;
   const int64_t tn = cdiv(g.N, dual ? gk::BNC : 2 * gk::BNC);
@@ -507,8 +502,6 @@ static GemmPlan gemm_plan(const Gemm& g) {
   }
   return best;
 }
-
-bool gemm_few_form(const Gemm& g) { return gemm_plan(g).mt == 0; }
 
 size_t gemm_ws_bytes(const Gemm& g) {
   const GemmPlan p = gemm_plan(g);

@@ -56,7 +56,12 @@ struct Gemm {
 // sizes alone (and whether a is K-major).
 size_t gemm_ws_bytes(const Gemm& g);
 int gemm_run(const Gemm& g, void* ws, cudaStream_t s);
-bool gemm_few_form(const Gemm& g);  // it takes the form of gemm_few.cu
+// How a product is cut: mt accumulators of 256 rows to a tile, or 0: the form of gemm_few.cu
+// with nt tokens to a tile; `splits` ranges of K.
+struct GemmPlan {
+  int mt, splits, nt;
+};
+GemmPlan gemm_plan(const Gemm& g);  // by the kind, the sizes and a.k_major alone
 
 // The form with swapped roles (gemm_few.cu): its estimated time, tile and cut, and the run.
 double few_estimate(const Gemm& g, int* nt, int* splits);

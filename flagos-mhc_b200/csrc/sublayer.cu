@@ -186,18 +186,33 @@ static size_t gemm_room(std::initializer_list<Gemm> gs) {
   for (const Gemm& g : gs) n = std::max(n, gemm_ws_bytes(g));
   return n;
 }
+// The matrix products of the operators, as enum mhc_product names them.
+static Gemm product_of(int32_t which, int64_t T, int64_t D, int64_t F) {
+  switch (which) {
+    case MHC_PRODUCT_GATE_UP: return product(kEpiGated, true, T, F, D);
+    case MHC_PRODUCT_GATED_GRAD_HIDDEN: return product(kEpiGatedBwd, true, T, F, D);
+    case MHC_PRODUCT_GATED_GRAD_X: return product(kEpiLinear, true, T, D, F, F);
+    case MHC_PRODUCT_GRAD_X: return product(kEpiLinear, true, T, D, F);
+    case MHC_PRODUCT_GRAD_WEIGHT: return product(kEpiLinear, false, F, D, T);
+    default: return product(kEpiLinear, true, T, F, D);
+  }
+}
 static size_t linear_fwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 || gemv_takes(T, F, D) ? 0 : gemm_room({product(kEpiLinear, true, T, F, D)});
+  return T == 0 || gemv_takes(T, F, D) ? 0 : gemm_room({product_of(MHC_PRODUCT_LINEAR, T, D, F)});
 }
 static size_t linear_bwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 ? 0 : gemm_room({product(kEpiLinear, true, T, D, F), product(kEpiLinear, false, F, D, T)});
+  return T == 0 ? 0 : gemm_room({product_of(MHC_PRODUCT_GRAD_X, T, D, F),
+                                 product_of(MHC_PRODUCT_GRAD_WEIGHT, T, D, F)});
 }
 static size_t ffn_fwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 || gemv_takes(T, F, D) ? 0 : gemm_room({product(kEpiGated, true, T, F, D), product(kEpiLinear, true, T, D, F)});
+  return T == 0 || gemv_takes(T, F, D) ? 0 : gemm_room({product_of(MHC_PRODUCT_GATE_UP, T, D, F),
+                                                        product_of(MHC_PRODUCT_LINEAR, T, F, D)});
 }
 static size_t ffn_bwd_room(int64_t T, int64_t D, int64_t F) {
-  return T == 0 ? 0 : gemm_room({product(kEpiGatedBwd, true, T, F, D), product(kEpiLinear, true, T, D, F, F),
-                                 product(kEpiLinear, false, F, D, T), product(kEpiLinear, false, D, F, T)});
+  return T == 0 ? 0 : gemm_room({product_of(MHC_PRODUCT_GATED_GRAD_HIDDEN, T, D, F),
+                                 product_of(MHC_PRODUCT_GATED_GRAD_X, T, D, F),
+                                 product_of(MHC_PRODUCT_GRAD_WEIGHT, T, D, F),
+                                 product_of(MHC_PRODUCT_GRAD_WEIGHT, T, F, D)});
 }
 
 // Runs a product whose output's rows may be unaligned: then it goes to a packed copy first, for
@@ -205,7 +220,7 @@ static size_t ffn_bwd_room(int64_t T, int64_t D, int64_t F) {
 // us by the copy).  The copy's room is taken from the Carver and free again afterwards.
 static int run_product(Gemm* g, void* room, Carver c, cudaStream_t s) {
   EpiParams& e = g->epi;
-  if (gemm_few_form(*g) || operand_aligned({e.out, e.ld_out, true})) return gemm_run(*g, room, s);
+  if (gemm_plan(*g).mt == 0 || operand_aligned({e.out, e.ld_out, true})) return gemm_run(*g, room, s);
   void *out = e.out, *z = e.z;
   const int64_t ld = e.ld_out;
   e.out = c.take(packed_bytes(g->M, g->N));
@@ -241,6 +256,24 @@ using namespace mhc;
   } while (0)
 
 extern "C" {
+
+int mhc_sublayer_plan(int32_t which, int64_t T, int64_t D, int64_t F, int32_t* form, int32_t* tile,
+                      int32_t* cuts) {
+  if (sub_check(T, D, F, MHC_BF16, MHC_ACT_NONE) != MHC_OK || T == 0 || which < MHC_PRODUCT_LINEAR ||
+      which > MHC_PRODUCT_GATED_GRAD_X || !form || !tile || !cuts)
+    return MHC_ERR_INVALID_ARGUMENT;
+  if ((which == MHC_PRODUCT_LINEAR || which == MHC_PRODUCT_GATE_UP) && gemv_takes(T, F, D)) {
+    *form = MHC_FORM_STREAM;
+    *tile = T <= 8 ? 8 : 16;
+    *cuts = 1;
+    return MHC_OK;
+  }
+  const GemmPlan p = gemm_plan(product_of(which, T, D, F));
+  *form = p.mt == 0 ? MHC_FORM_CLUSTER : MHC_FORM_PAIR;
+  *tile = p.mt == 0 ? p.nt : 256 * p.mt;
+  *cuts = p.splits;
+  return MHC_OK;
+}
 
 size_t mhc_linear_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
                                       int32_t unaligned) {

@@ -367,6 +367,32 @@ int mhc_layer_norm_bwd(const void* x, int64_t x_stride, const float* weight,
                        float* grad_weight, float* grad_bias, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* The matrix products of the linear layer and the gated block.  The gated
+ * block's down projection is MHC_PRODUCT_LINEAR with D and F exchanged, its
+ * weight gradients are MHC_PRODUCT_GRAD_WEIGHT (the down projection's with D and
+ * F exchanged). */
+enum mhc_product {
+  MHC_PRODUCT_LINEAR = 0,            /* x weight^T, (T,D) by (F,D)             */
+  MHC_PRODUCT_GRAD_X = 1,            /* gz weight                              */
+  MHC_PRODUCT_GRAD_WEIGHT = 2,       /* gz^T x                                 */
+  MHC_PRODUCT_GATE_UP = 3,           /* x w_gate^T and x w_up^T                */
+  MHC_PRODUCT_GATED_GRAD_HIDDEN = 4, /* grad_y w_down, to the grads of gate, up */
+  MHC_PRODUCT_GATED_GRAD_X = 5       /* gg w_gate + gu w_up                    */
+};
+enum mhc_form {
+  MHC_FORM_STREAM = 0,  /* weights streamed past up to `tile` tokens          */
+  MHC_FORM_CLUSTER = 1, /* tiles of 128 features by `tile` tokens             */
+  MHC_FORM_PAIR = 2     /* CTA pairs, tiles of `tile` rows of the output      */
+};
+
+/*
+ * Which kernel form a product takes on the current device (148 multiprocessors
+ * are assumed where there is none), and into how many ranges it cuts the summed
+ * dimension: for measurements and tests.  No device work.
+ */
+int mhc_sublayer_plan(int32_t product, int64_t T, int64_t D, int64_t F,
+                      int32_t* form, int32_t* tile, int32_t* cuts);
+
 /* Bytes of device workspace mhc_linear_fwd needs (may be 0). */
 size_t mhc_linear_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F,
                                       int32_t dtype, int32_t unaligned);
