@@ -155,6 +155,16 @@ struct Kahan {
     s = t;
   }
 };
+// The same for terms that may be infinite: the compensation turns an infinite sum into NaN, so the
+// plain sum is kept beside it and stands where the compensated one is not finite.
+struct KahanInf : Kahan {
+  float plain = 0.f;
+  __device__ __forceinline__ void add(float v) {
+    Kahan::add(v);
+    plain += v;
+  }
+  __device__ __forceinline__ float value() const { return isfinite(s) ? s : plain; }
+};
 __device__ __forceinline__ float4 kahan_add4(Kahan* k, float4 v) {
   k[0].add(v.x); k[1].add(v.y); k[2].add(v.z); k[3].add(v.w);
   return make_float4(k[0].s, k[1].s, k[2].s, k[3].s);

@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(32 * kLnSegs)
   __shared__ float sum[kLnSegs][33];
   const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5;
   const int64_t d = (int64_t)blockIdx.x * 32 + lane;
-  Kahan k;
+  KahanInf k;
   if (d < 2 * D) {
     const int i0 = blocks * seg / kLnSegs, i1 = blocks * (seg + 1) / kLnSegs;
     for (int i = i0; i < i1; i += 16) {
@@ -509,13 +509,13 @@ __global__ void __launch_bounds__(32 * kLnSegs)
       for (int j = 0; j < 16; ++j) k.add(v[j]);
     }
   }
-  sum[seg][lane] = k.s;
+  sum[seg][lane] = k.value();
   __syncthreads();
   if (seg == 0 && d < 2 * D) {
-    Kahan t;
+    KahanInf t;
 #pragma unroll
     for (int i = 0; i < kLnSegs; ++i) t.add(sum[i][lane]);
-    (d < D ? gw : gb - D)[d] = t.s;
+    (d < D ? gw : gb - D)[d] = t.value();
   }
 }
 

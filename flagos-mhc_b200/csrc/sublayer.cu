@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(256)
   __shared__ float sum[8][33];
   const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5;
   const int64_t f = (int64_t)blockIdx.x * 32 + lane;
-  Kahan k;
+  KahanInf k;
   if (f < F) {
     const int i0 = ranges * seg / 8, i1 = ranges * (seg + 1) / 8;
     for (int i = i0; i < i1; i += 8) {
@@ -99,13 +99,13 @@ __global__ void __launch_bounds__(256)
       for (int j = 0; j < 8; ++j) k.add(v[j]);
     }
   }
-  sum[seg][lane] = k.s;
+  sum[seg][lane] = k.value();
   __syncthreads();
   if (seg == 0 && f < F) {
-    Kahan t;
+    KahanInf t;
 #pragma unroll
     for (int i = 0; i < 8; ++i) t.add(sum[i][lane]);
-    st1<E>(gb + f, t.s);
+    st1<E>(gb + f, t.value());
   }
 }
 

@@ -120,3 +120,27 @@ def test_a_hosts_own_context_stays_current():
     th.start()
     th.join()
     assert seen == {"made": 0, "status": 0, "kept": True}
+
+
+@pytest.mark.parametrize("T", [1, 40, 3000])
+def test_sums_over_tokens_with_infinite_terms(T):
+    """One infinite gradient makes the sums of its column infinite, two of both signs NaN."""
+    D = F = 72
+    inf = float("inf")
+    x, w, gy = rnd(T, D, seed=1), rnd(F, D, seed=2), rnd(T, F, seed=3)
+    at = sorted({0, T // 2, T - 1})
+    for k, t in enumerate(at):
+        gy[t, k] = inf
+        gy[t, 8 + k] = -inf
+    gy[at[0], 20], gy[at[-1], 20] = inf, -inf
+    gb = M.mhc_linear_backward(x, w, None, gy, need_x_grad=False, need_weight_grad=False)[2]
+    want = gy.double().sum(0)
+    o = M.mhc_layer_norm(x, need_backward=True)
+    gw, gbn = M.mhc_layer_norm_backward(x, None, o["mean"], o["rstd"], gy)[1:]
+    xh = (x.double() - o["mean"].double()[:, None]) * o["rstd"].double()[:, None]
+    wantw = (gy.double() * xh).sum(0)
+    for got, ref in ((gb, want), (gbn, want), (gw, wantw)):
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        assert torch.equal(torch.isinf(got), torch.isinf(ref))
+        odd = torch.isinf(ref)
+        assert torch.equal(got[odd].double(), ref[odd])
