@@ -5,9 +5,10 @@
 
 namespace mhc {
 
-// expf / division are the fast intrinsics (a few ulp of fp32, against outputs that keep 8 or
-// 11 bits).  The sigmoid forms keep their relative accuracy in the negative tail, where
-// 1 + tanh or 1 + erf would cancel.
+// exp and division are the fast intrinsics, against outputs that keep 8 or 11 bits: exp(x) is off
+// by 2 + 1.2 |x| units in the last place, so a few where the functions are of any size and about 1e-5
+// relative at the far negative end.  The sigmoid forms keep their relative accuracy in the negative
+// tail, where 1 + tanh or 1 + erf would cancel; below -87.3 the sigmoid (1e-38 and less) is 0.
 __device__ __forceinline__ float sigmoid_fast(float z) {
   return __fdividef(1.f, 1.f + __expf(-z));
 }

@@ -15,12 +15,13 @@ def act(name, z):
         p = torch.sigmoid(z)
         return z * p, p * (1 + z * (1 - p))
     if name == "gelu":
-        cdf = torch.special.ndtr(z)
+        cdf = 0.5 * torch.erfc(-z / math.sqrt(2))   # 1 + erf would cancel in the negative tail
         return z * cdf, cdf + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    # 0.5 (1 + tanh(u)) = sigmoid(2u), which does not cancel in the negative tail
     c = math.sqrt(2 / math.pi)
-    t = torch.tanh(c * (z + 0.044715 * z ** 3))
-    return 0.5 * z * (1 + t), \
-        0.5 * (1 + t) + 0.5 * z * (1 - t * t) * c * (1 + 3 * 0.044715 * z * z)
+    u = 2 * c * (z + 0.044715 * z ** 3)
+    p, q = torch.sigmoid(u), torch.sigmoid(-u)
+    return z * p, p + z * p * q * 2 * c * (1 + 3 * 0.044715 * z * z)
 
 
 def layer_norm(x, weight, bias, eps):
