@@ -52,15 +52,6 @@ struct GemmWalk {
 };
 
 namespace tc2 {
-__device__ __forceinline__ uint32_t cta_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // address of the leader CTA's copy of a shared variable
 __device__ __forceinline__ uint32_t leader_addr(const void* p) {
   uint32_t r;
@@ -142,9 +133,8 @@ struct StoreTma {
   }
 };
 
-// tile index -> tile row and column: GROUP row tiles walk all column tiles together, so the
-// tiles in flight share their operands in L2
-// Unit i is tile i % tiles of K range i / tiles.
+// Unit u is tile u % tiles of K range u / tiles.  GROUP row tiles walk all column tiles together,
+// so that the tiles in flight share their operands in L2.
 struct Unit {
   int32_t mt, nt, split, kb0, kb1;
 };
@@ -182,7 +172,7 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = tc2::cta_rank();
+  const uint32_t rank = tc::cta_rank();
   const bool leader = rank == 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
@@ -207,7 +197,7 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
   }
   tc::tc_fence_before();
   __syncthreads();
-  tc2::cluster_sync();  // both CTAs' barriers are initialised
+  tc::cluster_sync();  // both CTAs' barriers are initialised
   tc::tc_fence_after();
   const uint32_t tmem = *(volatile uint32_t*)&tmem_slot;
   pdl_enter();
@@ -432,7 +422,7 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
   if (*abort_flag && threadIdx.x == 0) flag_timeout();
   tc::tc_fence_before();
   __syncthreads();
-  tc2::cluster_sync();  // neither CTA leaves while the other may still signal it
+  tc::cluster_sync();  // neither CTA leaves while the other may still signal it
   if (warp == 1) {
     tc::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");

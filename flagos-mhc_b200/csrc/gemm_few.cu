@@ -35,15 +35,6 @@ struct FewWalk {
   int32_t tiles_n, tiles_m, nk1, nk, splits;
 };
 
-__device__ __forceinline__ uint32_t few_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void few_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
   float4 v;
   uint32_t a;
@@ -70,7 +61,7 @@ __global__ void __launch_bounds__(fk::THREADS, 1)
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = w.splits > 1 ? few_rank() : 0;
+  const uint32_t rank = w.splits > 1 ? tc::cta_rank() : 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < R::STAGES; ++i) {
       tc::mbar_init(&full[i], 1);
@@ -191,7 +182,7 @@ __global__ void __launch_bounds__(fk::THREADS, 1)
   }
   tc::tc_fence_before();
   if (w.splits > 1)
-    few_cluster_sync();
+    tc::cluster_sync();
   else
     __syncthreads();
   // each CTA of the cluster: its tokens, 8 features to a thread
@@ -225,7 +216,7 @@ __global__ void __launch_bounds__(fk::THREADS, 1)
   }
   if (*abort_flag && threadIdx.x == 0) flag_timeout();
   if (w.splits > 1)
-    few_cluster_sync();  // the others may still read this CTA's accumulators
+    tc::cluster_sync();  // the others may still read this CTA's accumulators
   else
     __syncthreads();
   if (warp == 1) {
