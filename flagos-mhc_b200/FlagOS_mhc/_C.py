@@ -103,6 +103,8 @@ _SIGS = {
                                          _vp, _vp, _vp, _sz, _vp]),
 }
 
+MHC_GATE_UP_F32 = 0x100  # beside a dtype: the gated block's kept gate and up are fp32
+
 # activations of the linear layer and the gated feed-forward block (enum mhc_act)
 _ACT = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 

@@ -175,8 +175,9 @@ class MhcGatedFfnFn(torch.autograd.Function):
     false."""
 
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, activation, keep=True):
-        out = mhc_gated_ffn(x, w_gate, w_up, w_down, activation=activation, need_backward=keep)
+    def forward(ctx, x, w_gate, w_up, w_down, activation, keep=True, kept_dtype=torch.float32):
+        out = mhc_gated_ffn(x, w_gate, w_up, w_down, activation=activation, need_backward=keep,
+                            kept_dtype=kept_dtype)
         if keep:
             ctx.save_for_backward(x, w_gate, w_up, w_down, out["gate"], out["up"])
         ctx.activation = activation
@@ -186,11 +187,11 @@ class MhcGatedFfnFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_y):
         return mhc_gated_ffn_backward(*ctx.saved_tensors, grad_y, activation=ctx.activation,
-                                      need_grads=ctx.needs_input_grad[:4]) + (None, None)
+                                      need_grads=ctx.needs_input_grad[:4]) + (None,) * 3
 
 
-def mhc_gated_ffn_fn(x, w_gate, w_up, w_down, activation="silu"):
+def mhc_gated_ffn_fn(x, w_gate, w_up, w_down, activation="silu", kept_dtype=torch.float32):
     """Autograd-aware mhc_gated_ffn. Returns y.  gate and up are written only if a gradient is
-    wanted."""
+    wanted, in ``kept_dtype`` (as in :func:`FlagOS_mhc.mhc_gated_ffn`)."""
     return MhcGatedFfnFn.apply(x, w_gate, w_up, w_down, activation,
-                               _graph_wanted(x, w_gate, w_up, w_down))
+                               _graph_wanted(x, w_gate, w_up, w_down), kept_dtype)

@@ -4,7 +4,7 @@ from __future__ import annotations
 import torch
 
 from . import _C
-from .mhc_gated_ffn import _check_ffn
+from .mhc_gated_ffn import _check_ffn, _kept_flag
 from .mhc_linear import _act_ref, _matrix_dtype
 
 
@@ -12,7 +12,8 @@ def mhc_gated_ffn_backward(x, w_gate, w_up, w_down, gate, up, grad_y, activation
                            need_grads=(True, True, True, True)):
     """Returns (grad_x, grad_w_gate, grad_w_up, grad_w_down) in x's dtype.
 
-    ``gate`` and ``up`` (T, F) are the forward's (``need_backward=True``).  One kernel
+    ``gate`` and ``up`` (T, F) are the forward's (``need_backward=True``), both float32 or
+    both x's dtype.  One kernel
     forms grad_y w_down and, in its epilogue, the gradients of gate and up and the hidden
     product; grad_x is one product over both projections.  ``need_grads``: the outputs that
     are wanted; the others are None.
@@ -24,7 +25,12 @@ def mhc_gated_ffn_backward(x, w_gate, w_up, w_down, gate, up, grad_y, activation
         assert tuple(t.shape) == (T, F), f"{name} shape {tuple(t.shape)} != {(T, F)}"
     _C.require_cuda(x, w_gate, w_up, w_down, gate, up, grad_y)
     code = _matrix_dtype(x)
-    _C.require_same("mhc_gated_ffn_backward", x, w_gate, w_up, w_down, gate, up, grad_y)
+    _C.require_same("mhc_gated_ffn_backward", x, w_gate, w_up, w_down, grad_y)
+    _C.require_same("mhc_gated_ffn_backward", gate, up)
+    if gate.device != x.device:
+        raise RuntimeError(f"FlagOS_mhc.mhc_gated_ffn_backward: tensors on {x.device} and "
+                           f"{gate.device}")
+    code |= _kept_flag("mhc_gated_ffn_backward", gate.dtype, x)
     need_grads = tuple(need_grads)
     if not any(need_grads):
         return (None,) * 4

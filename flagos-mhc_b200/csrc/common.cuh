@@ -176,7 +176,7 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// 16-bit element conversions (round to nearest even)
+// Element conversions (to 16 bits: round to nearest even)
 template <typename E> __device__ __forceinline__ E to_e(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 to_e<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
@@ -184,6 +184,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 to_e<__nv_bfloat16>(float v
 template <> __device__ __forceinline__ __half to_e<__half>(float v) { return __float2half_rn(v); }
 __device__ __forceinline__ float from_e(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float from_e(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_e<float>(float v) { return v; }
+__device__ __forceinline__ float from_e(float v) { return v; }
 
 // fp16 tensor-core operands: values are multiplied by 2^s before their hi/lo split, with
 // 2^s chosen from their maximum magnitude (bits of a non-negative float) so that the

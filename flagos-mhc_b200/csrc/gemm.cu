@@ -113,23 +113,28 @@ struct StoreTma {
   int32_t row0;   // of the warp's chunk
   int lane;
   int next = 0;
-  template <typename E, int NC>
-  __device__ __forceinline__ void put(int which, void*, int64_t, int64_t, int64_t col, int, int,
+  template <typename E, int NC>  // the type in memory; a chunk is one box of 16 bits, two of fp32
+  __device__ __forceinline__ void put(int which, void*, int64_t, int64_t, int64_t col, int n, int,
                                       const float* f) {
-    static_assert(NC == 32, "a box is 32 columns wide");
-    if (lane == 0) tc::bulk_wait_read<1>();  // the store before the last has read this box
-    __syncwarp();
-    char* b = box + next * 2048 + lane * 64;
+    static_assert(NC == 32, "a chunk is 32 columns wide");
+    constexpr int P = 16 / sizeof(E), PER = 4 * P;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<uint4*>(b + ((j ^ ((lane >> 1) & 3)) << 4)) = narrow<E>(f + 8 * j);
-    tc::fence_proxy_async();
-    __syncwarp();
-    if (lane == 0) {
-      tc::tma_store_2d(&maps[which], box + next * 2048, (int32_t)col, row0);
-      tc::bulk_commit_group();
+    for (int c = 0; c < NC; c += PER) {
+      if (c >= n) break;                       // a box that starts past the last column
+      if (lane == 0) tc::bulk_wait_read<1>();  // the store before the last has read this box
+      __syncwarp();
+      char* b = box + next * 2048 + lane * 64;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint4*>(b + ((j ^ ((lane >> 1) & 3)) << 4)) = narrow<E>(f + c + P * j);
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        tc::tma_store_2d(&maps[which], box + next * 2048, (int32_t)col + c, row0);
+        tc::bulk_commit_group();
+      }
+      next ^= 1;
     }
-    next ^= 1;
   }
 };
 
@@ -347,9 +352,22 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
       const int64_t row = row0 + lane, rrow = row < w.M ? row : w.M - 1;
       st.row0 = (int32_t)row0;
       const int64_t col0 = (int64_t)u.nt * (dual ? BNC : 2 * BNC) + col_off;
-      // kEpiGatedBwd reads gate and up: a chunk ahead, the first before the products are done
+      // kEpiGatedBwd reads gate and up: a chunk ahead, the first before the products are done.
+      // kEpiGatedBwd32, whose chunk would take 64 registers, asks for the tile's lines in L2 instead.
       constexpr bool ahead = KIND == kEpiGatedBwd;
       Raw32 pre[ahead ? 4 : 1];
+      if constexpr (KIND == kEpiGatedBwd32) {
+        if (w.splits == 1) {
+          const float* pg = reinterpret_cast<const float*>(epi.gate) + rrow * epi.ld_gu + col0;
+          const float* pu = reinterpret_cast<const float*>(epi.up) + rrow * epi.ld_gu + col0;
+#pragma unroll
+          for (int c = 0; c < COLS; c += 32) {  // 128 bytes
+            if (col0 + c >= w.N) break;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(pg + c));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(pu + c));
+          }
+        }
+      }
       auto fetch = [&](int c) {
         if constexpr (ahead) {
           if (epi.vec == 2 && w.splits == 1 && col0 + c + 32 <= w.N) {
@@ -504,7 +522,8 @@ int epi_vec(const EpiParams& e) {
   for (const void* p : {(const void*)e.out, e.bias, e.res, (const void*)e.z, (const void*)e.gate,
                         (const void*)e.up, (const void*)e.gg, (const void*)e.gu})
     bits |= reinterpret_cast<uintptr_t>(p);
-  for (int64_t ld : {e.ld_out, e.ld_res, e.ld_gu, e.ld_g}) bits |= (uintptr_t)ld * 2;
+  for (int64_t ld : {e.ld_out, e.ld_res, e.gu32 ? 2 * e.ld_gu : e.ld_gu, e.ld_g})
+    bits |= (uintptr_t)ld * 2;
   return (bits & 31) == 0 ? 2 : (bits & 15) == 0 ? 1 : 0;
 }
 
@@ -536,16 +555,19 @@ static int gemm_launch(const Gemm& g, int splits, float* part, cudaStream_t s) {
   for (CUtensorMap& o : m.out) o = m.a;
   if (splits == 1 && g.epi.vec) {
     const EpiParams& e = g.epi;
-    auto out = [&](int i, const void* p, int64_t ld) {
+    auto out = [&](int i, const void* p, int64_t ld, bool f32 = false) {
       if (!p || st) return;
-      st = make_tmap_2d(&m.out[i], p, g.dtype == MHC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                        2, g.N, g.M, ld * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+      const int size = f32 ? 4 : 2;
+      st = make_tmap_2d(&m.out[i], p,
+                        f32                  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : g.dtype == MHC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                             : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                        size, g.N, g.M, ld * size, 64 / size, 32, CU_TENSOR_MAP_SWIZZLE_64B);
     };
     out(0, e.out, e.ld_out);
     if (KIND == kEpiLinear) out(1, e.z, e.ld_out);
-    if (KIND == kEpiGated) out(1, e.gate, e.ld_gu), out(2, e.up, e.ld_gu);
-    if (KIND == kEpiGatedBwd) out(1, e.gg, e.ld_g), out(2, e.gu, e.ld_g);
+    if (KIND == kEpiGated) out(1, e.gate, e.ld_gu, e.gu32), out(2, e.up, e.ld_gu, e.gu32);
+    if (KIND == kEpiGatedBwd || KIND == kEpiGatedBwd32) out(1, e.gg, e.ld_g), out(2, e.gu, e.ld_g);
     if (st) return st;
   }
   GemmWalk w;
@@ -611,6 +633,7 @@ static int gemm_typed(const Gemm& g, void* ws, cudaStream_t s) {
   // the operands' orders that the operators meet
   if (g.kind == kEpiGated) return gemm_kind<E, kEpiGated, true, true>(g, ws, s);
   if (g.kind == kEpiGatedBwd) return gemm_kind<E, kEpiGatedBwd, true, false>(g, ws, s);
+  if (g.kind == kEpiGatedBwd32) return gemm_kind<E, kEpiGatedBwd32, true, false>(g, ws, s);
   if (!g.a.k_major) return gemm_kind<E, kEpiLinear, false, false>(g, ws, s);
   return g.b.k_major ? gemm_kind<E, kEpiLinear, true, true>(g, ws, s)
                      : gemm_kind<E, kEpiLinear, true, false>(g, ws, s);

@@ -19,22 +19,24 @@ enum EpiKind {
   kEpiLinear = 0,    // y = act(acc + bias) + residual, z = acc + bias
   kEpiGated = 1,     // two products: gate, up; h = act(gate) * up
   kEpiGatedBwd = 2,  // acc = gh; from gate and up: gg, gu and h
+  kEpiGatedBwd32 = 3,  // the same, gate and up in fp32 (EpiParams::gu32)
 };
 
 struct EpiParams {
   int act = MHC_ACT_NONE;
-  // kEpiLinear: out = y.  kEpiGated, kEpiGatedBwd: out = h
+  // kEpiLinear: out = y.  The others: out = h
   void* out = nullptr;
   int64_t ld_out = 0;
   const void* bias = nullptr;
   const void* res = nullptr;
   int64_t ld_res = 0;
   void* z = nullptr;  // packed like out
-  // kEpiGated: outputs or null.  kEpiGatedBwd: inputs
+  // kEpiGated: outputs or null.  kEpiGatedBwd(32): inputs.  fp32 if gu32, else the operands' type
   void* gate = nullptr;
   void* up = nullptr;
   int64_t ld_gu = 0;
-  // kEpiGatedBwd: outputs
+  int gu32 = 0;
+  // kEpiGatedBwd(32): outputs
   void* gg = nullptr;
   void* gu = nullptr;
   int64_t ld_g = 0;
@@ -82,7 +84,7 @@ int epi_vec(const EpiParams& e);
 
 // ---------------------------------------------------------------- epilogue
 // A thread owns a row here, so every access of a warp touches 32 rows: 32-byte accesses (whole
-// sectors) halve the requests where the rows allow them.
+// sectors) halve the requests where the rows allow them.  E: the type in memory, 16 bits or fp32.
 struct alignas(32) Raw32 {
   uint4 a, b;
 };
@@ -102,17 +104,18 @@ __device__ __forceinline__ void st_row32(void* p, const uint4& a, const uint4& b
 }
 template <typename E, int NC>
 __device__ __forceinline__ void row_load(const void* base, int64_t off, int n, int vec, float* f) {
+  constexpr int P = 16 / sizeof(E);
   const E* p = reinterpret_cast<const E*>(base) + off;
-  if (NC % 16 == 0 && vec == 2 && n == NC) {
+  if (NC % (2 * P) == 0 && vec == 2 && n == NC) {
 #pragma unroll
-    for (int i = 0; i < NC; i += 16) {
+    for (int i = 0; i < NC; i += 2 * P) {
       const Raw32 r = ld_row32(p + i);
       widen<E>(r.a, f + i);
-      widen<E>(r.b, f + i + 8);
+      widen<E>(r.b, f + i + P);
     }
-  } else if (NC % 8 == 0 && vec && n == NC) {
+  } else if (NC % P == 0 && vec && n == NC) {
 #pragma unroll
-    for (int i = 0; i < NC; i += 8) widen<E>(*reinterpret_cast<const uint4*>(p + i), f + i);
+    for (int i = 0; i < NC; i += P) widen<E>(*reinterpret_cast<const uint4*>(p + i), f + i);
   } else {
 #pragma unroll
     for (int i = 0; i < NC; ++i) f[i] = i < n ? from_e(p[i]) : 0.f;
@@ -120,13 +123,14 @@ __device__ __forceinline__ void row_load(const void* base, int64_t off, int n, i
 }
 template <typename E, int NC>
 __device__ __forceinline__ void row_store(void* base, int64_t off, int n, int vec, const float* f) {
+  constexpr int P = 16 / sizeof(E);
   E* p = reinterpret_cast<E*>(base) + off;
-  if (NC % 16 == 0 && vec == 2 && n == NC) {
+  if (NC % (2 * P) == 0 && vec == 2 && n == NC) {
 #pragma unroll
-    for (int i = 0; i < NC; i += 16) st_row32(p + i, narrow<E>(f + i), narrow<E>(f + i + 8));
-  } else if (NC % 8 == 0 && vec && n == NC) {
+    for (int i = 0; i < NC; i += 2 * P) st_row32(p + i, narrow<E>(f + i), narrow<E>(f + i + P));
+  } else if (NC % P == 0 && vec && n == NC) {
 #pragma unroll
-    for (int i = 0; i < NC; i += 8) *reinterpret_cast<uint4*>(p + i) = narrow<E>(f + i);
+    for (int i = 0; i < NC; i += P) *reinterpret_cast<uint4*>(p + i) = narrow<E>(f + i);
   } else {
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -144,12 +148,13 @@ struct StoreRows {
 };
 
 // Roundings.  Everything here is fp32; what is stored in 16 bits is stored so because it is an operand
-// of the next product, which the tensor cores take in 16 bits (h, gg, gu), or kept by the caller from
-// the forward to the backward (z, gate, up: in 32 bits they would double the largest tensors that a
-// training step keeps).  The backward's activation is of the kept, rounded gate.  Each adds an
-// independent half step: the gated block's output is off by 2.35e-3 in the 2-norm in bf16 and its
-// gradients by 3.5e-3, where one rounding of the output alone makes 1.66e-3; the linear layer's
-// gradients by 1.45 times the rounding.  In fp16 h passes the type's range where act(gate) up does.
+// of the next product, which the tensor cores take in 16 bits (h, gg, gu), or because the caller keeps
+// it so from the forward to the backward (z; gate and up on request, which halves the largest tensors
+// that a training step keeps; in fp32 otherwise).  The backward's activation is of the kept gate.  Each
+// rounding adds an independent half step: where that of the output alone makes 1.66e-3 in the 2-norm
+// in bf16, the gated block's output and its gradients are off by 2.35e-3, the gradients by 3.5e-3 with
+// gate and up in 16 bits; the linear layer's gradients by 1.45 times the output's.  In fp16 h passes
+// the type's range where act(gate) up does.
 //
 // n <= NC valid columns of one row, starting at col (a multiple of 8).  acc: the product;
 // acc2: the second product of kEpiGated; for kEpiGatedBwd gate and up where they were loaded
@@ -174,7 +179,10 @@ __device__ __forceinline__ void epi_act(const EpiParams& e, int64_t row, int64_t
     }
     st.template put<E, NC>(0, e.out, row, e.ld_out, col, n, e.vec, acc);
   } else if constexpr (KIND == kEpiGated) {
-    if (e.gate) {
+    if (e.gate && e.gu32) {
+      st.template put<float, NC>(1, e.gate, row, e.ld_gu, col, n, e.vec, acc);
+      st.template put<float, NC>(2, e.up, row, e.ld_gu, col, n, e.vec, acc2);
+    } else if (e.gate) {
       st.template put<E, NC>(1, e.gate, row, e.ld_gu, col, n, e.vec, acc);
       st.template put<E, NC>(2, e.up, row, e.ld_gu, col, n, e.vec, acc2);
     }
@@ -182,13 +190,14 @@ __device__ __forceinline__ void epi_act(const EpiParams& e, int64_t row, int64_t
     for (int i = 0; i < NC; ++i) v[i] = act_fwd<ACT>(acc[i]) * acc2[i];
     st.template put<E, NC>(0, e.out, row, e.ld_out, col, n, e.vec, v);
   } else {
+    using G = std::conditional_t<KIND == kEpiGatedBwd32, float, E>;
     float u[NC];
     if (acc2) {  // loaded ahead: gate in v's place, then up
 #pragma unroll
       for (int i = 0; i < NC; ++i) v[i] = acc2[i], u[i] = acc2[NC + i];
     } else {
-      row_load<E, NC>(e.gate, row * e.ld_gu + col, n, e.vec, v);
-      row_load<E, NC>(e.up, row * e.ld_gu + col, n, e.vec, u);
+      row_load<G, NC>(e.gate, row * e.ld_gu + col, n, e.vec, v);
+      row_load<G, NC>(e.up, row * e.ld_gu + col, n, e.vec, u);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {

@@ -334,6 +334,7 @@ template <typename E>
 static int few_typed(const Gemm& g, int nt, int splits, cudaStream_t s) {
   if (g.kind == kEpiGated) return few_kind<E, kEpiGated, true>(g, nt, splits, s);
   if (g.kind == kEpiGatedBwd) return few_kind<E, kEpiGatedBwd, false>(g, nt, splits, s);
+  if (g.kind == kEpiGatedBwd32) return few_kind<E, kEpiGatedBwd32, false>(g, nt, splits, s);
   return g.b.k_major ? few_kind<E, kEpiLinear, true>(g, nt, splits, s)
                      : few_kind<E, kEpiLinear, false>(g, nt, splits, s);
 }

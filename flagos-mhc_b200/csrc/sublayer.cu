@@ -186,6 +186,12 @@ static size_t gemm_room(std::initializer_list<Gemm> gs) {
   for (const Gemm& g : gs) n = std::max(n, gemm_ws_bytes(g));
   return n;
 }
+// dtype with the flag on the kept gate and up taken off
+static bool take_gate_up_f32(int32_t* dtype) {
+  const bool f32 = (*dtype & MHC_GATE_UP_F32) != 0;
+  *dtype &= ~MHC_GATE_UP_F32;
+  return f32;
+}
 // The matrix products of the operators, as enum mhc_product names them.
 static Gemm product_of(int32_t which, int64_t T, int64_t D, int64_t F) {
   switch (which) {
@@ -401,6 +407,7 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight, int64_t 
 
 size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
                                          int32_t unaligned) {
+  take_gate_up_f32(&dtype);
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
   Carver c{nullptr};
   c.take(packed_bytes(T, F));  // h
@@ -419,6 +426,7 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
                       int64_t w_down_stride, int64_t T, int64_t D, int64_t F, int32_t dtype,
                       int32_t act, void* y, void* gate, void* up, int64_t gate_up_stride,
                       void* workspace, size_t workspace_bytes, void* stream) {
+  const bool gate_up_f32 = take_gate_up_f32(&dtype);
   RETURN_IF(sub_check(T, D, F, dtype, act));
   if (x_stride < D || w_gate_stride < D || w_up_stride < D || w_down_stride < F ||
       (gate == nullptr) != (up == nullptr) || (gate && gate_up_stride < F))
@@ -453,6 +461,7 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
   g.b2 = ou;
   g.epi.act = act; g.epi.out = h; g.epi.ld_out = ldh;
   g.epi.gate = gate; g.epi.up = up; g.epi.ld_gu = gate ? gate_up_stride : 0;
+  g.epi.gu32 = gate_up_f32;
   RETURN_IF(few ? gemv_run(g, s) : gemm_run(g, room, s));
   Gemm d;
   d.dtype = dtype;
@@ -465,6 +474,7 @@ int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate, int64
 
 size_t mhc_gated_ffn_bwd_workspace_bytes(int64_t T, int64_t D, int64_t F, int32_t dtype,
                                          int32_t unaligned) {
+  take_gate_up_f32(&dtype);
   if (sub_check(T, D, F, dtype, 0) != MHC_OK) return 0;
   Carver c{nullptr};
   for (int i = 0; i < 3; ++i) c.take(packed_bytes(T, F));  // gg, gu, h
@@ -485,6 +495,7 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
                       int64_t T, int64_t D, int64_t F, int32_t dtype, int32_t act, void* grad_x,
                       void* grad_w_gate, void* grad_w_up, void* grad_w_down, void* workspace,
                       size_t workspace_bytes, void* stream) {
+  const bool gate_up_f32 = take_gate_up_f32(&dtype);
   RETURN_IF(sub_check(T, D, F, dtype, act));
   if (x_stride < D || w_gate_stride < D || w_up_stride < D || w_down_stride < F ||
       gate_up_stride < F || grad_y_stride < D)
@@ -519,7 +530,7 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
   RETURN_IF(aligned_operand(&od, D, F, &c, s));
   {
     Gemm g;  // gh = grad_y w_down, then gg, gu and h in its epilogue
-    g.kind = kEpiGatedBwd;
+    g.kind = gate_up_f32 ? kEpiGatedBwd32 : kEpiGatedBwd;
     g.dtype = dtype;
     g.M = T; g.N = F; g.K = D;
     g.a = oy;
@@ -527,6 +538,7 @@ int mhc_gated_ffn_bwd(const void* x, int64_t x_stride, const void* w_gate, int64
     g.epi.act = act;
     g.epi.gate = const_cast<void*>(gate); g.epi.up = const_cast<void*>(up);
     g.epi.ld_gu = gate_up_stride;
+    g.epi.gu32 = gate_up_f32;
     g.epi.gg = gg; g.epi.gu = gu; g.epi.ld_g = ld;
     g.epi.out = h; g.epi.ld_out = ld;
     RETURN_IF(gemm_run(g, room, s));

@@ -429,6 +429,15 @@ int mhc_linear_bwd(const void* x, int64_t x_stride, const void* weight,
                    void* grad_x, void* grad_weight, void* grad_bias,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * The gated block keeps gate and up from the forward to the backward.  They are
+ * dtype, or fp32 where the entry points (and their workspace queries) are given
+ * dtype | MHC_GATE_UP_F32: twice the bytes, and gradients off by 1.4 times the
+ * rounding of the output alone in place of 2.1 times.  Both calls of a pair
+ * take the same.
+ */
+#define MHC_GATE_UP_F32 0x100
+
 /* Bytes of device workspace mhc_gated_ffn_fwd needs. */
 size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F,
                                          int32_t dtype, int32_t unaligned);
@@ -438,7 +447,8 @@ size_t mhc_gated_ffn_fwd_workspace_bytes(int64_t T, int64_t D, int64_t F,
  *   gate = x w_gate^T;  up = x w_up^T;  h = act(gate) * up;  y = h w_down^T
  * x: (T,D); w_gate, w_up: (F,D); w_down: (D,F); y: (T,D) packed; gate, up:
  * (T,F), rows gate_up_stride apart, or NULL (both or neither; kept for the
- * backward).  All dtype.  h is rounded to dtype: it is a matrix operand.
+ * backward).  All dtype, gate and up as above.  h is rounded to dtype: it is a
+ * matrix operand.
  */
 int mhc_gated_ffn_fwd(const void* x, int64_t x_stride, const void* w_gate,
                       int64_t w_gate_stride, const void* w_up,

@@ -53,3 +53,9 @@ def test_gated_forms(i, dt):
     again = M.mhc_gated_ffn_backward(x, wg, wu, wd, o["gate"].contiguous(), o["up"].contiguous(), gy,
                                      activation=name)
     assert same(again, g)
+    # gate and up kept in 16 bits: rounded once, and read back as the same values
+    h = M.mhc_gated_ffn(x, wg, wu, wd, activation=name, need_backward=True, kept_dtype=dt)
+    assert same(h.values(), [o["y"], o["gate"].to(dt), o["up"].to(dt)])
+    g = M.mhc_gated_ffn_backward(x, wg, wu, wd, h["gate"], h["up"], gy, activation=name)
+    for gate, up in ((h["gate"].float(), h["up"].float()), (h["gate"].contiguous(), h["up"].contiguous())):
+        assert same(M.mhc_gated_ffn_backward(x, wg, wu, wd, gate, up, gy, activation=name), g)

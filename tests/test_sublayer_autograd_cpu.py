@@ -16,7 +16,8 @@ def kept(monkeypatch):
         seen.append(need_backward)
         return M.mhc_linear_ref(x, weight, bias, residual, activation)
 
-    def gated(x, w_gate, w_up, w_down, activation="silu", need_backward=False):
+    def gated(x, w_gate, w_up, w_down, activation="silu", need_backward=False,
+              kept_dtype=torch.float32):
         seen.append(need_backward)
         return M.mhc_gated_ffn_ref(x, w_gate, w_up, w_down, activation)
 

@@ -68,6 +68,24 @@ def test_gated_ffn_takes_the_queried_workspace(T, D, F, pad):
                                    gd, WS, n, None))
 
 
+def test_gate_and_up_in_fp32_are_a_flag_on_the_dtype():
+    L, f32 = _C.lib(), _C.MHC_GATE_UP_F32
+    for dt in (1, 2):
+        n = L.mhc_gated_ffn_fwd_workspace_bytes(40, 136, 264, dt | f32, 0)
+        assert n == L.mhc_gated_ffn_fwd_workspace_bytes(40, 136, 264, dt, 0) > 0
+        passes(L.mhc_gated_ffn_fwd(P, 136, P, 136, P, 136, P, 264, 40, 136, 264, dt | f32, 4, P, P, P, 264,
+                                   WS, n, None))
+        n = L.mhc_gated_ffn_bwd_workspace_bytes(40, 136, 264, dt | f32, 0)
+        assert n == L.mhc_gated_ffn_bwd_workspace_bytes(40, 136, 264, dt, 0) > 0
+        passes(L.mhc_gated_ffn_bwd(P, 136, P, 136, P, 136, P, 264, P, P, 264, P, 136, 40, 136, 264, dt | f32,
+                                   4, P, P, P, P, WS, n, None))
+    # the operands stay 16 bits, and no other operator takes the flag
+    assert L.mhc_gated_ffn_fwd(P, 16, P, 16, P, 16, P, 8, 4, 16, 8, f32, 4, P, P, P, 8, WS, 1 << 20,
+                               None) == _C.MHC_ERR_UNSUPPORTED_DTYPE
+    assert L.mhc_linear_fwd(P, 16, P, 16, None, None, 0, 4, 16, 8, 2 | f32, 4, P, None, None, 0,
+                            None) == _C.MHC_ERR_UNSUPPORTED_DTYPE
+
+
 def test_a_backward_without_outputs_has_nothing_to_do():
     """No device, no workspace: the calls return before either is asked for."""
     L = _C.lib()
