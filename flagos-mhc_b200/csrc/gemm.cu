@@ -353,22 +353,19 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
       st.row0 = (int32_t)row0;
       const int64_t col0 = (int64_t)u.nt * (dual ? BNC : 2 * BNC) + col_off;
       // kEpiGatedBwd reads gate and up: a chunk ahead, the first before the products are done.
-      // kEpiGatedBwd32, whose chunk would take 64 registers, asks for the tile's lines in L2 instead.
+      // kEpiGatedBwd32, whose chunk would take 64 registers, asks for its lines in L2 instead (T=4096,
+      // 4096/16384: 455 us; 492 us with the whole tile's lines at its start, some of which were gone
+      // again when they were read).
       constexpr bool ahead = KIND == kEpiGatedBwd;
       Raw32 pre[ahead ? 4 : 1];
-      if constexpr (KIND == kEpiGatedBwd32) {
-        if (w.splits == 1) {
-          const float* pg = reinterpret_cast<const float*>(epi.gate) + rrow * epi.ld_gu + col0;
-          const float* pu = reinterpret_cast<const float*>(epi.up) + rrow * epi.ld_gu + col0;
-#pragma unroll
-          for (int c = 0; c < COLS; c += 32) {  // 128 bytes
-            if (col0 + c >= w.N) break;
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(pg + c));
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(pu + c));
+      auto fetch = [&](int c) {
+        if constexpr (KIND == kEpiGatedBwd32) {
+          if (w.splits == 1 && col0 + c < w.N) {  // a chunk's row is 128 bytes
+            const int64_t at = rrow * epi.ld_gu + col0 + c;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const float*>(epi.gate) + at));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const float*>(epi.up) + at));
           }
         }
-      }
-      auto fetch = [&](int c) {
         if constexpr (ahead) {
           if (epi.vec == 2 && w.splits == 1 && col0 + c + 32 <= w.N) {
             const E* pg = reinterpret_cast<const E*>(epi.gate) + rrow * epi.ld_gu + col0 + c;
@@ -427,6 +424,7 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
               epi_chunk<E, KIND, 32>(epi, rrow, col0 + c, n, acc, more, st);
             }
           } else {
+            if (c + 32 < COLS) fetch(c + 32);
             epi_chunk<E, KIND, 32>(epi, rrow, col0 + c, n, acc, more, st);
           }
         } else if (row < w.M) {
