@@ -9,8 +9,9 @@ namespace mhc {
 
 // ------------------------------------------------------------------ gz and grad_bias
 // gz = grad_y * act'(z), rounded to dtype as the operand of both products that follow, and, per row
-// range, the column sums of the unrounded gz: bound by HBM.  A block takes 256 columns of a row range, 8 to a thread (a 16-byte pack where the rows
-// allow it), its warps every eighth row; their sums are added in order.
+// range, the column sums of the unrounded gz: bound by HBM.  A block takes 256 columns of a row
+// range, 8 to a thread (a 16-byte pack where the rows allow it), its warps every eighth row; their
+// sums are added in order.
 // About 4096 blocks, of at least 32 rows (65536 x 4096, silu: 271 us with 256 ranges, 306 us with
 // 64; two or four rows of a warp at once took 380 and 473 us).
 static int gz_ranges(int64_t T, int64_t F) {
