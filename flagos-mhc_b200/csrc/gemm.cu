@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                        ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2], tdone;
-  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t tmem_slot, filled;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
         if (!more) break;
         if (!tc::mbar_wait_warp(&empty[s], ph, abort_flag)) {
           more = false;
+          if (issue) filled = tc::fills_at(s, ph);
           break;
         }
         const uint32_t bar = bar0 + s * 8;
@@ -269,6 +270,7 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
         }
         __syncwarp();
         advance();
+        if (!more && issue) filled = tc::fills_at(s + 1, ph);
       }
     }
   } else if (warp == 1) {
@@ -439,6 +441,8 @@ __global__ void __launch_bounds__(gk::THREADS, 1)
   if (*abort_flag && threadIdx.x == 0) flag_timeout();
   tc::tc_fence_before();
   __syncthreads();
+  // the loads of both CTAs are counted on the leader's barriers
+  if (leader && *abort_flag && threadIdx.x == 0) tc::drain(full, STAGES, filled);
   tc::cluster_sync();  // neither CTA leaves while the other may still signal it
   if (warp == 1) {
     tc::tc_fence_after();

@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(fk::THREADS, 1)
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                        ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t full[R::STAGES], empty[R::STAGES], done;
-  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t tmem_slot, filled;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(fk::THREADS, 1)
         if (kb >= kb1) break;
         if (!tc::mbar_wait_warp(&empty[s], ph, abort_flag)) {
           kb = kb1;
+          if (issue) filled = tc::fills_at(s, ph);
           break;
         }
         char* sa = smem + s * R::STAGE_BYTES;
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(fk::THREADS, 1)
           tc::tma_load_2d(sb, second ? &maps.b3 : &maps.b, &full[s], k0, t0);
         }
         __syncwarp();
-        ++kb;
+        if (++kb == kb1 && issue) filled = tc::fills_at(s + 1, ph);
       }
     }
   } else if (warp == 1) {
@@ -214,7 +215,10 @@ __global__ void __launch_bounds__(fk::THREADS, 1)
     epi_chunk<E, KIND, 8>(epi, t0 + tok, f0 + f, left < 8 ? (int)left : 8, v[0],
                           W == 2 ? v[W - 1] : nullptr);
   }
-  if (*abort_flag && threadIdx.x == 0) flag_timeout();
+  if (*abort_flag && threadIdx.x == 0) {
+    flag_timeout();
+    tc::drain(full, R::STAGES, filled);
+  }
   if (w.splits > 1)
     tc::cluster_sync();  // the others may still read this CTA's accumulators
   else

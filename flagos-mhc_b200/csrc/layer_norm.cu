@@ -206,16 +206,19 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
   __shared__ __align__(8) uint64_t full[kLnMaxStages];
   __shared__ float red[2][2][WARPS], n_of[WARPS];
   __shared__ int abort_word;
+  __shared__ uint32_t filled;  // thread 0's: the parity of each stage's last fill
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t row_bytes = (uint32_t)D * sizeof(E);
   if (tid == 0) {
     for (int i = 0; i < stages; ++i) tc::mbar_init(&full[i], 1);
     abort_word = 0;
+    filled = ~0u;
     tc::fence_barrier_init();
   }
   __syncthreads();
   pdl_enter();
   auto fetch = [&](int64_t t, int s) {
+    filled ^= 1u << s;
     tc::mbar_arrive_expect_tx(&full[s], row_bytes);
     tc::bulk_load(ring + (size_t)s * row_bytes, x + t * xs, row_bytes, &full[s]);
   };
@@ -283,6 +286,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
     }
     if (++s == stages) s = 0, ph ^= 1;
   }
+  if (tid == 0 && *(volatile int*)&abort_word) tc::drain(full, stages, filled);
 }
 
 // The part of the backward that follows the loads: sums over the row, grad_x, and with PARAMS
@@ -394,16 +398,19 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
   __shared__ __align__(8) uint64_t full[kLnMaxStages];
   __shared__ __align__(16) float red[2][2][WARPS];
   __shared__ int abort_word;
+  __shared__ uint32_t filled;  // thread 0's: the parity of each stage's last fill
   const int tid = threadIdx.x;
   const uint32_t row_bytes = (uint32_t)D * sizeof(E);
   if (tid == 0) {
     for (int i = 0; i < stages; ++i) tc::mbar_init(&full[i], 1);
     abort_word = 0;
+    filled = ~0u;
     tc::fence_barrier_init();
   }
   __syncthreads();
   pdl_enter();
   auto fetch = [&](int64_t t, int s) {
+    filled ^= 1u << s;
     char* dst = ring + (size_t)s * 2 * row_bytes;
     tc::mbar_arrive_expect_tx(&full[s], 2 * row_bytes);
     tc::bulk_load(dst, x + t * xs, row_bytes, &full[s]);
@@ -486,6 +493,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
     r1 = r2;
   }
   if constexpr (PARAMS) ln_bwd_partials<PN, GT, V>(part, tid, D, aw, ab);
+  if (tid == 0 && *(volatile int*)&abort_word) tc::drain(full, stages, filled);
 }
 
 // Sums of the blocks' partials: 32 columns per block, 16 contiguous ranges of partials added

@@ -67,6 +67,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
   *abort = 1;
   return false;
 }
+// After a wait has given up: waits, again with a limit, for the loads that may still be on their
+// way into a ring's stages, so that none lands in shared memory that another CTA has been given.
+// Bit s of `parity`: that of stage s's last fill, 1 where it has had none.  A loader that stops
+// before stage s of a pass, in which it waits for empty stages with parity ph (1 in the first), has
+// filled the stages before s with ph ^ 1 and the others with ph.
+__device__ __forceinline__ uint32_t fills_at(int s, uint32_t ph) {
+  return ph ? ~0u << s : (1u << s) - 1;
+}
+__device__ __forceinline__ void drain(uint64_t* full, int stages, uint32_t parity) {
+  for (int s = 0; s < stages; ++s) {
+    volatile int own = 0;
+    mbar_wait(&full[s], (parity >> s) & 1, &own, 1u << 20);
+  }
+}
 
 // ---------------------------------------------------------------- TMA (tiled, no multicast)
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar,
